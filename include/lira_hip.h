@@ -318,6 +318,107 @@ int lira_select_probes(const float *scores, int64_t n, int64_t n_centroids, int 
 int lira_order_probes(int32_t *probe, int64_t n, int64_t max_probe, const float *key, int64_t n_centroids,
                       void *stream);
 
+/* ------------------------------------------- microscaled 4-bit floats */
+/* element types of the entries below */
+#define LIRA_DTYPE_F32 0
+#define LIRA_DTYPE_BF16 1
+#define LIRA_DTYPE_F16 2
+/* activations of the product's epilogue */
+#define LIRA_ACT_NONE 0
+#define LIRA_ACT_RELU 1
+#define LIRA_ACT_SIGMOID 2
+/*
+ * Rows of 4-bit floats (sign, 2 exponent bits, 1 mantissa bit: 0, .5, 1, 1.5,
+ * 2, 3, 4, 6) in blocks of 32 along the row, one power-of-two scale a block.
+ * No counterpart in the reference, which keeps x_d in fp32 (search.cpp:387-403):
+ * a row of d = 128 takes 68 bytes instead of 512.
+ *
+ * Layout: rows are padded with zeros to planes of 128 elements, P = ceil(k / 128).
+ *   codes   (P, plane_rows, 64) bytes, 16-byte aligned: element 2i of a plane in
+ *           the low half of byte i (a code is sign << 3 | exponent << 1 | mantissa)
+ *   scales  (P, plane_rows, 4) bytes, 4-byte aligned: block b's scale is
+ *           2^(scales[b] - 127); 255 makes the block NaN
+ * plane_rows >= the rows used, so a range of rows of a larger array can be passed.
+ *
+ * lira_mx4_quantize packs x (n, k), row stride ld elements, any alignment:
+ *   block scale = 2^max(floor(log2 max|x|) - 2, -127), element = x / scale to
+ *   nearest (ties to the even code), saturated at 6.  A block of zeros has scale
+ *   byte 0; one that holds Inf or NaN has 255 and codes 0.
+ * lira_mx4_dequantize is the inverse (exact in fp32, one rounding to the 16-bit types).
+ * All entries: device pointers, stream-ordered, asynchronous, capturable, no
+ * state between calls; every output element is written by one call in a fixed
+ * order of operations, so results do not vary from run to run.
+ */
+int lira_mx4_quantize(const void *x, int dtype, int64_t n, int64_t k, int64_t ld, uint8_t *codes,
+                      uint8_t *scales, int64_t plane_rows, void *stream);
+int lira_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t plane_rows, int64_t n,
+                        int64_t k, void *out, int dtype, int64_t ld, void *stream);
+/*
+ * out[i, j] = act(alpha * sum_l a[i, l] b[j, l] + bias[j]) of two packed arrays,
+ * a (m, k) and b (n, k): fp32 sums on the matrix cores, rounded once to out_dtype.
+ * bias: fp32 (n) or NULL.  out (m, n), row stride ldo elements; elements outside
+ * it are left as they are.  m <= 1048560.  The 4-bit form of the products that
+ * lira_centroid_gemm computes in fp32 (search.cpp:220-235) and of the probing
+ * model's layers (model_probing.py:33-39).
+ */
+int lira_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, int64_t a_plane_rows, int64_t m,
+                    const uint8_t *b_codes, const uint8_t *b_scales, int64_t b_plane_rows, int64_t n,
+                    int64_t k, float alpha, const float *bias, int act, void *out, int out_dtype,
+                    int64_t ldo, void *stream);
+/*
+ * The same with rows of x (m, k) that are packed on the way (exactly as
+ * lira_mx4_quantize packs them).  workspace: device, 16-byte aligned, at least
+ * lira_mx4_linear_workspace_size() bytes (0 for some shapes: NULL is then fine);
+ * one per concurrent call.
+ */
+int lira_mx4_linear_workspace_size(int64_t m, int64_t n, int64_t k, size_t *bytes);
+int lira_mx4_linear(const void *x, int dtype, int64_t m, int64_t k, int64_t ldx, const uint8_t *b_codes,
+                    const uint8_t *b_scales, int64_t b_plane_rows, int64_t n, float alpha, const float *bias,
+                    int act, void *out, int out_dtype, int64_t ldo, void *workspace, size_t workspace_bytes,
+                    void *stream);
+
+/* ------------------------------------------------------- distillation */
+/*
+ * Loss of a student's outputs against a teacher's top outputs, and its gradient:
+ * how a probing model (model_probing.py:41-54 trains it on kNN partition labels)
+ * learns from the top of an exact ranking or of a larger model.  For row r, with
+ * logits z (vocab), teacher entries (ids[j], teacher[j]), j < top, temperature T:
+ *   log p_j = teacher[j] / T - L,  L = logsumexp over the row's entries, or
+ *             teacher_lse[r] where given (the teacher's logsumexp of ALL its
+ *             logits / T: then s = sum_j p_j < 1)
+ *   log q_v = z_v / T - logsumexp_v(z_v / T)
+ *   loss[r] = T^2 sum_{p_j > 0} p_j (log p_j - log q_ids[j])
+ *   dz[r,v] = row_scale[r * scale_stride] T (s q_v - sum_{j: ids[j] = v} p_j)
+ * ids < 0 are unused entries; an id may occur more than once.  A row in which no
+ * entry counts has loss 0 and gradient 0.  z_v = -inf is a masked output: q_v = 0
+ * (the loss is +inf where an entry of p > 0 names it).  NaN or +inf among the z,
+ * NaN among the entries, or an id >= vocab makes the row's loss and gradient NaN.
+ *   z, dz     dtype, (rows, vocab), row strides ldz / ldd elements, any
+ *             alignment; dz may be z itself (ldd = ldz), else must not overlap it
+ *   ids       int32 or int64 (ids_bits), (rows, top); teacher fp32 (rows, top);
+ *             1 <= top <= 1024
+ *   loss      fp32 (rows)
+ *   stats     fp32 (rows, 2) out or NULL: the student's logsumexp and s, for
+ *             lira_distill_topk_backward on the same inputs
+ *   dz        NULL: the loss alone.  scale_stride 0: row_scale holds one factor
+ *             for all rows; row_scale NULL: 1
+ * fp32 sums in a fixed order (results do not vary from run to run), dz rounded
+ * once.  Device pointers, stream-ordered, asynchronous, capturable.
+ * lira_distill_reduce: out[0] = sum of loss, or (mean) the mean over the rows
+ * that count; out[1] = the factor of every row's gradient, 1 or 1 / count.
+ */
+int lira_distill_topk(const void *z, int dtype, int64_t rows, int64_t vocab, int64_t ldz, const void *ids,
+                      int ids_bits, const float *teacher, int64_t top, float temperature,
+                      const float *teacher_lse, float *loss, float *stats, const float *row_scale,
+                      int64_t scale_stride, void *dz, int64_t ldd, void *stream);
+int lira_distill_topk_backward(const void *z, int dtype, int64_t rows, int64_t vocab, int64_t ldz,
+                               const void *ids, int ids_bits, const float *teacher, int64_t top,
+                               float temperature, const float *teacher_lse, const float *stats,
+                               const float *row_scale, int64_t scale_stride, void *dz, int64_t ldd,
+                               void *stream);
+int lira_distill_reduce(const float *loss, const float *stats, int64_t rows, int mean, float *out,
+                        void *stream);
+
 /* -------------------------------------------------------------- scan */
 /*
  * Batched candidate scan + exact top-k over the probed buckets.

@@ -1,0 +1,86 @@
+// lira_mx4.hpp -- device helpers of the microscaled 4-bit format (lira_mx4.hip).
+//
+// A block is 32 consecutive elements of a row: 32 codes of 4 bits (sign, 2 exponent bits, 1
+// mantissa bit: 0, .5, 1, 1.5, 2, 3, 4, 6) and one scale 2^(s - 127), s a byte (255: NaN).
+// A plane is 128 elements = 4 blocks = 64 bytes of codes and 4 of scales; planes are the
+// outer dimension, so the 16 x 128 fragment of v_mfma_scale_f32_16x16x128_f8f6f4 is 1 KiB
+// of consecutive codes: lane l holds block l / 16 of row l % 16 (16 bytes) and its scale.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace lira {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// element types of lira_hip.h's LIRA_DTYPE_*
+struct F32 {
+    typedef float T;
+    static __device__ __forceinline__ float up(float v) { return v; }
+    static __device__ __forceinline__ float down(float v) { return v; }
+};
+struct BF16 {
+    typedef __bf16 T;
+    static __device__ __forceinline__ float up(__bf16 v) { return (float)v; }
+    static __device__ __forceinline__ __bf16 down(float v) { return (__bf16)v; }  // to nearest, ties to even
+};
+struct F16 {
+    typedef _Float16 T;
+    static __device__ __forceinline__ float up(_Float16 v) { return (float)v; }
+    static __device__ __forceinline__ _Float16 down(float v) { return (_Float16)v; }
+};
+
+// |v| as an integer: orders like |v| and puts Inf and NaN above every number
+__device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+// the scale byte of a block whose largest magnitude has these bits: exponent - 2 (6 = 1.5 * 2^2
+// is the largest element), not below 2^-127; 255 where the block holds Inf or NaN
+__device__ __forceinline__ uint32_t scale_code(uint32_t m) {
+    const uint32_t e = m >> 23;
+    return e == 255 ? 255u : e < 2 ? 0u : e - 2;
+}
+// the operand form of v_cvt_scalef32_*: only the exponent field counts
+__device__ __forceinline__ float scale_operand(uint32_t code) { return __uint_as_float(code << 23); }
+
+// 8 floats -> 8 codes, element 0 in the low 4 bits; v / scale to nearest even, saturated at 6
+__device__ __forceinline__ uint32_t to_codes(const float (&v)[8], float scale) {
+    uint32_t r = 0;
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], scale, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], scale, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[4], v[5], scale, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[6], v[7], scale, 3);
+    return r;
+}
+
+// the number a code stands for times 2^(s - 127); exact in fp32 (at most 2 mantissa bits)
+__device__ __forceinline__ float from_code(uint32_t c, uint32_t s) {
+    const uint32_t a = c & 7u;
+    float v = a < 2 ? 0.5f * (float)a : __uint_as_float(((a >> 1) + 126u) << 23 | (a & 1u) << 22);
+    v = (c & 8u) ? -v : v;
+    return s == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(v, (int)s - 127);
+}
+
+// 8 consecutive elements of a row from element j (zeros past the row's end); VEC: the row's
+// first element and the row stride are multiples of 16 bytes
+template <class D, bool VEC>
+__device__ __forceinline__ void load8(const typename D::T *row, int64_t j, int64_t k, float (&v)[8]) {
+    typedef typename D::T T;
+    if (VEC && j + 8 <= k) {
+        struct alignas(16) V {
+            T e[8];
+        };
+        const V t = *reinterpret_cast<const V *>(row + j);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = D::up(t.e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = j + i < k ? D::up(row[j + i]) : 0.0f;
+    }
+}
+
+}  // namespace lira

@@ -34,6 +34,13 @@ LIRA_PROBE_THRESHOLD_GE = 1
 LIRA_PROBE_THRESHOLD_GT = 2
 LIRA_PROBE_BY_SCORE = 16
 
+LIRA_DTYPE_F32 = 0
+LIRA_DTYPE_BF16 = 1
+LIRA_DTYPE_F16 = 2
+LIRA_ACT_NONE = 0
+LIRA_ACT_RELU = 1
+LIRA_ACT_SIGMOID = 2
+
 _STATUS = {
     -1: "EINVAL",
     -2: "ERANGE",
@@ -73,6 +80,17 @@ SIGNATURES = {
     "lira_select_probes": (_INT, [_P, _I64, _I64, _INT, _F, _I64, _P, _P, _P]),
     "lira_order_probes": (_INT, [_P, _I64, _I64, _P, _I64, _P]),
     "lira_merge_shards": (_INT, [_P, _P, _I64, _I64, _I64, _INT, _INT, _P, _P, _P]),
+    "lira_mx4_quantize": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _P, _I64, _P]),
+    "lira_mx4_dequantize": (_INT, [_P, _P, _I64, _I64, _I64, _P, _INT, _I64, _P]),
+    "lira_mx4_matmul": (_INT, [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _F, _P, _INT, _P, _INT, _I64, _P]),
+    "lira_mx4_linear_workspace_size": (_INT, [_I64, _I64, _I64, ctypes.POINTER(_SZ)]),
+    "lira_mx4_linear": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _P, _I64, _I64, _F, _P, _INT, _P, _INT, _I64, _P,
+                               _SZ, _P]),
+    "lira_distill_topk": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _INT, _P, _I64, _F, _P, _P, _P, _P, _I64, _P, _I64,
+                                 _P]),
+    "lira_distill_topk_backward": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _INT, _P, _I64, _F, _P, _P, _P, _I64, _P,
+                                          _I64, _P]),
+    "lira_distill_reduce": (_INT, [_P, _P, _I64, _INT, _P, _P]),
     "lira_scan_workspace_size": (_INT, [_P, _I64, _I64, _I64, ctypes.c_uint, ctypes.POINTER(_SZ)]),
     "lira_scan_topk": (_INT, [_P, _P, _I64, _P, _I64, _I64, ctypes.c_uint, _P, _P, _P, _P, _SZ, _P]),
     "lira_scan_describe": (_INT, [_P, _I64, _I64, _I64, ctypes.c_uint, ctypes.c_char_p, _SZ]),

@@ -1,0 +1,235 @@
+"""Microscaled 4-bit floats: packed rows, and their products on the matrix cores.
+
+Stored vectors and the probing model's layers in 4.25 bits an element: 32 elements share a
+power-of-two scale (include/lira_hip.h has the layout and the rounding).  A row of d = 128
+takes 68 bytes, where the reference's fp32 copy (search.cpp:387-403) takes 512.
+
+* ``mx4_quantize`` / ``MX4Tensor.dequantize``   pack rows and read them back
+* ``mx4_matmul``   act(alpha * A B^T + bias) of two packed arrays
+* ``mx4_linear``   the same with fp32 / bf16 / fp16 rows that are packed on the way
+
+All of them run on the current stream (or ``stream=``), allocate nothing that outlives the call but
+their results, and can be captured into a graph.  They have no gradient: an input that asks
+for one is refused.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+
+from . import _lib
+
+DTYPES = {torch.float32: _lib.LIRA_DTYPE_F32, torch.bfloat16: _lib.LIRA_DTYPE_BF16,
+          torch.float16: _lib.LIRA_DTYPE_F16}
+ACTIVATIONS = {None: _lib.LIRA_ACT_NONE, "relu": _lib.LIRA_ACT_RELU, "sigmoid": _lib.LIRA_ACT_SIGMOID}
+
+
+def on(device: torch.device, stream=None):
+    """The context a call runs in: the tensors' device, and ``stream`` as the current one, so that
+    whatever the call allocates belongs to the stream that uses it."""
+    if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
+        return torch.cuda.stream(stream)
+    if device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def check_rows(x, name: str, device=None) -> torch.Tensor:
+    """A 2-D device tensor of a float type the kernels read; copied only if its rows are not runs of
+    consecutive elements."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError(f"{name} must be a tensor on the GPU")
+    if x.dtype not in DTYPES:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, not {x.dtype}")
+    if x.dim() != 2:
+        raise ValueError(f"{name} must have 2 dimensions, not {x.dim()}")
+    if device is not None and x.device != device:
+        raise ValueError(f"{name} is on {x.device}, not on {device}")
+    return x
+
+
+def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """x with consecutive elements in its rows, and its row stride."""
+    n, k = x.shape
+    if x.stride(1) == 1 and (n <= 1 or x.stride(0) >= k):
+        return x, k if n <= 1 else x.stride(0)
+    x = x.contiguous()
+    return x, k
+
+
+def _no_grad(*tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("the 4-bit operators have no gradient: call them under torch.no_grad() or on detached tensors")
+
+
+class MX4Tensor:
+    """Packed rows: ``codes`` (P, n, 64) uint8, ``scales`` (P, n, 4) uint8, P = ceil(k / 128)
+    planes of 128 elements (include/lira_hip.h).  Row ranges ``t[lo:hi]`` are views."""
+
+    __slots__ = ("codes", "scales", "k", "plane_rows")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int):
+        k = int(k)
+        for t, w, name in ((codes, 64, "codes"), (scales, 4, "scales")):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 3 or t.shape[2] != w:
+                raise ValueError(f"{name} must be a (P, n, {w}) uint8 tensor on the GPU")
+        if k < 1 or codes.shape[0] != (k + 127) // 128:
+            raise ValueError(f"k = {k} needs {(max(k, 1) + 127) // 128} planes, codes have {codes.shape[0]}")
+        if codes.shape[:2] != scales.shape[:2] or codes.device != scales.device:
+            raise ValueError("codes and scales must have the same planes and rows, on one device")
+        rows = self._plane_rows(codes)
+        if rows is None or rows != self._plane_rows(scales) or codes.data_ptr() % 16 or scales.data_ptr() % 4:
+            codes, scales = codes.clone(memory_format=torch.contiguous_format), \
+                scales.clone(memory_format=torch.contiguous_format)
+            rows = codes.shape[1]
+        self.codes, self.scales, self.k, self.plane_rows = codes, scales, k, rows
+
+    @staticmethod
+    def _plane_rows(t: torch.Tensor):
+        p, n, w = t.shape
+        if t.is_contiguous():
+            return n
+        if t.stride(2) != 1 or (n > 1 and t.stride(1) != w):
+            return None
+        if p == 1:
+            return n
+        return t.stride(0) // w if t.stride(0) % w == 0 and t.stride(0) >= n * w else None
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.codes.shape[1], self.k
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def __len__(self) -> int:
+        return self.codes.shape[1]
+
+    def __getitem__(self, rows: slice) -> "MX4Tensor":
+        if not isinstance(rows, slice) or rows.step not in (None, 1):
+            raise TypeError("an MX4Tensor is cut by a range of rows, t[lo:hi]")
+        return MX4Tensor(self.codes[:, rows], self.scales[:, rows], self.k)
+
+    def dequantize(self, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
+                   stream=None) -> torch.Tensor:
+        """The rows as numbers, (n, k): exact in float32, rounded once to the 16-bit types."""
+        return mx4_dequantize(self, dtype, out, stream)
+
+
+def mx4_quantize(x: torch.Tensor, stream=None) -> MX4Tensor:
+    """Pack the rows of x (n, k), float32 / bfloat16 / float16 (lira_mx4_quantize)."""
+    x = check_rows(x, "x")
+    _no_grad(x)
+    n, k = x.shape
+    if k < 1:
+        raise ValueError("x must have at least one column")
+    p = (k + 127) // 128
+    with on(x.device, stream):
+        x, ld = _rows(x)
+        codes = torch.empty((p, n, 64), dtype=torch.uint8, device=x.device)
+        scales = torch.empty((p, n, 4), dtype=torch.uint8, device=x.device)
+        _lib.call("lira_mx4_quantize", x.data_ptr(), DTYPES[x.dtype], n, k, ld, codes.data_ptr(), scales.data_ptr(), n,
+                  _lib.stream_ptr())
+    return MX4Tensor(codes, scales, k)
+
+
+def _out(out, shape, dtype, device) -> torch.Tensor:
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if not isinstance(out, torch.Tensor) or out.device != device or out.dtype != dtype or tuple(out.shape) != shape:
+        raise ValueError(f"out must be a {shape} {dtype} tensor on {device}")
+    if shape[1] > 1 and out.stride(1) != 1 or shape[0] > 1 and out.stride(0) < shape[1]:
+        raise ValueError("out must have rows of consecutive elements that do not overlap")
+    return out
+
+
+def _ld(out: torch.Tensor) -> int:
+    return out.stride(0) if out.shape[0] > 1 else max(1, out.shape[1])
+
+
+def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
+                   stream=None) -> torch.Tensor:
+    """The rows of t as numbers (lira_mx4_dequantize)."""
+    if not isinstance(t, MX4Tensor):
+        raise ValueError("t must be an MX4Tensor")
+    if dtype not in DTYPES:
+        raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
+    with on(t.device, stream):
+        out = _out(out, t.shape, dtype, t.device)
+        _no_grad(out)
+        _lib.call("lira_mx4_dequantize", t.codes.data_ptr(), t.scales.data_ptr(), t.plane_rows, t.shape[0], t.k,
+                  out.data_ptr(), DTYPES[dtype], _ld(out), _lib.stream_ptr())
+    return out
+
+
+def _epilogue(w, bias, activation):
+    if not isinstance(w, MX4Tensor):
+        raise ValueError("the right operand must be an MX4Tensor (mx4_quantize packs one)")
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, not {activation!r}")
+    if bias is None:
+        return None, ACTIVATIONS[activation]
+    if not isinstance(bias, torch.Tensor) or bias.device != w.device or tuple(bias.shape) != (w.shape[0],) \
+            or not bias.is_floating_point():
+        raise ValueError(f"bias must be a ({w.shape[0]},) float tensor on {w.device}")
+    _no_grad(bias)
+    return bias, ACTIVATIONS[activation]
+
+
+def mx4_matmul(a: MX4Tensor, b: MX4Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+               alpha: float = 1.0, out_dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
+               stream=None) -> torch.Tensor:
+    """activation(alpha * a @ b.T + bias), (a rows, b rows) in out_dtype, sums in fp32
+    (lira_mx4_matmul).  activation: None, "relu" or "sigmoid"; bias (b rows,)."""
+    if not isinstance(a, MX4Tensor):
+        raise ValueError("the left operand must be an MX4Tensor (mx4_linear packs plain rows on the way)")
+    bias, act = _epilogue(b, bias, activation)
+    if a.k != b.k or a.device != b.device:
+        raise ValueError(f"a has {a.k} columns on {a.device}, b has {b.k} on {b.device}")
+    if out_dtype not in DTYPES:
+        raise ValueError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
+    m, n = a.shape[0], b.shape[0]
+    with on(a.device, stream):
+        bias = None if bias is None else bias.to(torch.float32).contiguous()
+        out = _out(out, (m, n), out_dtype, a.device)
+        _no_grad(out)
+        _lib.call("lira_mx4_matmul", a.codes.data_ptr(), a.scales.data_ptr(), a.plane_rows, m, b.codes.data_ptr(),
+                  b.scales.data_ptr(), b.plane_rows, n, a.k, float(alpha), _lib.ptr(bias), act, out.data_ptr(),
+                  DTYPES[out_dtype], _ld(out), _lib.stream_ptr())
+    return out
+
+
+def mx4_linear(x: torch.Tensor, w: MX4Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
+               alpha: float = 1.0, out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None,
+               stream=None) -> torch.Tensor:
+    """activation(alpha * Q(x) @ w.T + bias): the rows of x (m, k) are packed on the way, exactly as
+    mx4_quantize packs them (lira_mx4_linear).  The result has x's type unless out_dtype says otherwise."""
+    bias, act = _epilogue(w, bias, activation)
+    x = check_rows(x, "x", w.device)
+    _no_grad(x)
+    if x.shape[1] != w.k:
+        raise ValueError(f"x has {x.shape[1]} columns, w has {w.k}")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in DTYPES:
+        raise ValueError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
+    m, n = x.shape[0], w.shape[0]
+    need = ctypes.c_size_t()
+    _lib.call("lira_mx4_linear_workspace_size", m, n, w.k, ctypes.byref(need))
+    with on(x.device, stream):
+        x, ld = _rows(x)
+        bias = None if bias is None else bias.to(torch.float32).contiguous()
+        out = _out(out, (m, n), out_dtype, x.device)
+        _no_grad(out)
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
+        _lib.call("lira_mx4_linear", x.data_ptr(), DTYPES[x.dtype], m, w.k, ld, w.codes.data_ptr(),
+                  w.scales.data_ptr(), w.plane_rows, n, float(alpha), _lib.ptr(bias), act, out.data_ptr(),
+                  DTYPES[out_dtype], _ld(out), _lib.ptr(ws), need.value, _lib.stream_ptr())
+    return out
