@@ -390,16 +390,21 @@ int lira_mx4_linear(const void *x, int dtype, int64_t m, int64_t k, int64_t ldx,
  *   loss[r] = T^2 sum_{p_j > 0} p_j (log p_j - log q_ids[j])
  *   dz[r,v] = row_scale[r * scale_stride] T (s q_v - sum_{j: ids[j] = v} p_j)
  * ids < 0 are unused entries; an id may occur more than once.  A row in which no
- * entry counts has loss 0 and gradient 0.  z_v = -inf is a masked output: q_v = 0
- * (the loss is +inf where an entry of p > 0 names it).  NaN or +inf among the z,
- * NaN among the entries, or an id >= vocab makes the row's loss and gradient NaN.
+ * entry counts (all unused, or of p = 0) has loss 0 and gradient 0, whatever its
+ * logits.  z_v = -inf is a masked output: q_v = 0 (the loss is +inf where an entry
+ * of p > 0 names it).  NaN or +inf among the z, NaN among the used entries, or an
+ * id >= vocab makes the row's loss and gradient NaN.
  *   z, dz     dtype, (rows, vocab), row strides ldz / ldd elements, any
  *             alignment; dz may be z itself (ldd = ldz), else must not overlap it
  *   ids       int32 or int64 (ids_bits), (rows, top); teacher fp32 (rows, top);
  *             1 <= top <= 1024
  *   loss      fp32 (rows)
- *   stats     fp32 (rows, 2) out or NULL: the student's logsumexp and s, for
- *             lira_distill_topk_backward on the same inputs
+ *   stats     fp32 (rows, 4), 16-byte aligned, out or NULL: max z, log2 of the sum
+ *             of 2^((z - max) log2(e) / T), s, 0 -- for lira_distill_topk_backward
+ *             on the same inputs
+ *   workspace device, 16-byte aligned, at least lira_distill_workspace_size() bytes
+ *             (0 unless few long rows are split over the chip; NULL is then fine);
+ *             one per concurrent call
  *   dz        NULL: the loss alone.  scale_stride 0: row_scale holds one factor
  *             for all rows; row_scale NULL: 1
  * fp32 sums in a fixed order (results do not vary from run to run), dz rounded
@@ -410,7 +415,9 @@ int lira_mx4_linear(const void *x, int dtype, int64_t m, int64_t k, int64_t ldx,
 int lira_distill_topk(const void *z, int dtype, int64_t rows, int64_t vocab, int64_t ldz, const void *ids,
                       int ids_bits, const float *teacher, int64_t top, float temperature,
                       const float *teacher_lse, float *loss, float *stats, const float *row_scale,
-                      int64_t scale_stride, void *dz, int64_t ldd, void *stream);
+                      int64_t scale_stride, void *dz, int64_t ldd, void *workspace, size_t workspace_bytes,
+                      void *stream);
+int lira_distill_workspace_size(int64_t rows, int64_t vocab, int64_t top, int dtype, size_t *bytes);
 int lira_distill_topk_backward(const void *z, int dtype, int64_t rows, int64_t vocab, int64_t ldz,
                                const void *ids, int ids_bits, const float *teacher, int64_t top,
                                float temperature, const float *teacher_lse, const float *stats,

@@ -5,22 +5,36 @@
 //   log q_v = z_v / T - logsumexp_v(z_v / T),  s = sum_j p_j
 //   loss    = T^2 sum_{p_j > 0} p_j (log p_j - log q_{i_j})
 //   d/dz_v  = T (s q_v - sum_{j: i_j = v} p_j)
-// A row without a used entry has loss 0 and gradient 0.  z = -inf has q = 0.  NaN or +inf
-// among the z, or an id >= vocab, makes the whole row NaN.  Sums in fp32; the gradient is
-// rounded once, to the type of z.
+// A row in which no entry counts has loss 0 and gradient 0, whatever its logits.  z = -inf has
+// q = 0.  NaN or +inf among the z, NaN among the entries, or an id >= vocab makes the row NaN.
+//
+// Memory-bound: the loss reads z once, the gradient writes as much.  Everything is in powers of 2
+// of (z - max) c, c = log2(e) / T: one subtraction and one fma before the exp, no overflow where
+// z holds its type's lowest value.  Sums in fp32 in a fixed order.
+//
+// A group of NT threads works on a row (or a slice of it).  Thread u holds the 16-byte vectors u,
+// u + NT, ..: in registers (NV of them) where loss and gradient are wanted together, so that z is
+// read from memory once.  Rows need not be aligned: the vectors are of the row, not of memory.
+//
+// The teacher's entries change single places of the gradient.  The first wave puts each entry
+// into a list of the thread that stores its place (LDS); that thread stores the place once more
+// after its vectors -- its own stores to one address stay in order, so no barrier waits for them.
+#include <algorithm>
 #include <string>
 
+#include "lira_device.hpp"
 #include "lira_internal.hpp"
 #include "lira_mx4.hpp"
 
 namespace lira {
 
 static constexpr int kMaxTop = 1024;
-static constexpr float kLog2e = 1.44269504088896340736f;
+static constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
 struct DistillArgs {
     const void *z;
-    int64_t rows, vocab, ldz;
+    int64_t rows;
+    int64_t vocab, ldz;
     const void *ids;
     const float *tv;
     int top, ids64;
@@ -28,121 +42,357 @@ struct DistillArgs {
     float t;                   // temperature
     const float *row_scale;    // factor of each row's gradient: row_scale[r * scale_stride]; NULL: 1
     int64_t scale_stride;
-    float *loss;               // may be NULL
-    float *stats;              // (rows, 2): student logsumexp of z / T, s (0: no entry counts, NaN: the row is NaN)
-    void *dz;                  // NULL: loss alone
+    float *loss;
+    float *stats;  // (rows, 4): max z, log2 sum 2^((z - max) c), s (0: no entry counts, NaN: the row is NaN), 0
+    void *dz;
     int64_t ldd;
-    int mode;                  // 0: loss (and dz) from scratch; 1: dz alone, from stats
+    int slices;      // of a row, kSliceVecs vectors each (1: whole rows)
+    float2 *part;    // [rows][slices] (max, sum) of the slices
+    float *xs;       // [rows][top] the z that the entries name
 };
 
-// (max, sum of 2^((x - max) log2e)) pairs: joined as in a running softmax
-struct MS {
-    float m, s;
+enum Mode {
+    kLoss,   // loss and stats
+    kBoth,   // loss, stats and gradient
+    kGrad,   // gradient from stats
+    kPart,   // a slice's (max, sum) and, by slice 0, the entries' z
+    kJoin,   // the slices' joined: loss by slice 0, and the slice's gradient if wanted
 };
-__device__ __forceinline__ float e2(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
-__device__ __forceinline__ MS join(MS a, MS b) {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) return {m, a.s + b.s};  // (both sums are 0, or NaN)
-    return {m, a.s * e2(a.m - m) + b.s * e2(b.m - m)};
+
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int m = 1; m <= 32; m <<= 1) v = fmaxf(v, __uint_as_float(xor_u32(__float_as_uint(v), m)));
+    return v;
 }
-__device__ __forceinline__ MS add(MS a, float x) { return join(a, {x, x == -INFINITY ? 0.0f : x != x ? x : 1.0f}); }
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int m = 1; m <= 32; m <<= 1) v += __uint_as_float(xor_u32(__float_as_uint(v), m));
+    return v;
+}
 
+// 16 bytes of a row, at any alignment
 template <class D>
-__global__ __launch_bounds__(256) void k_distill(DistillArgs a) {
+struct Vec {
     typedef typename D::T T;
-    __shared__ float sm[4], ss[4], sp[kMaxTop], sx[kMaxTop];
-    __shared__ int64_t sid[kMaxTop];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int64_t r = blockIdx.x;
+    static constexpr int E = 16 / sizeof(T);
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const T *at) { __builtin_memcpy(w, at, 16); }
+    __device__ __forceinline__ void store(T *at) const { __builtin_memcpy(at, w, 16); }
+    __device__ __forceinline__ float get(int i) const {
+        if (sizeof(T) == 4) return __uint_as_float(w[i]);
+        const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+        T t;
+        __builtin_memcpy(&t, &h, sizeof(T) == 2 ? 2 : 0);
+        return D::up(t);
+    }
+    // (the passes over a row unpack anew: unpacked values kept from one to the next would take
+    // twice the registers that the row itself does)
+    __device__ __forceinline__ void forget() { asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3])); }
+    __device__ __forceinline__ void mask(bool there) {
+        constexpr uint32_t none = sizeof(T) == 4 ? 0xff800000u : D::kNegInf * 0x10001u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = there ? w[i] : none;
+    }
+    __device__ __forceinline__ float max() const {
+        float m = get(0);
+#pragma unroll
+        for (int i = 1; i < E; ++i) m = fmaxf(m, get(i));
+        return m;
+    }
+    __device__ __forceinline__ float sum(float m, float c) const {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) s += ex2((get(i) - m) * c);
+        return s;
+    }
+    __device__ __forceinline__ void grad(float m, float c, float l2, float f) {
+        T o[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] = D::down(f * ex2(fmaf(get(i) - m, c, -l2)));
+        __builtin_memcpy(w, o, 16);
+    }
+};
+
+static constexpr int kSliceVecs = 1024;  // 4 vectors a thread of 256
+
+template <class D, int NT, int NV, int KM, Mode MODE>
+__global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) {
+    typedef typename D::T T;
+    typedef Vec<D> V;
+    constexpr int E = V::E, G = NT < 256 ? 256 / NT : 1, NW = NT / 64, J = KM / 64;
+    constexpr bool kStats = MODE == kLoss || MODE == kBoth || MODE == kPart;
+    constexpr bool kDz = MODE == kBoth || MODE == kGrad || MODE == kJoin;
+    constexpr bool kEntries = MODE != kPart;
+    static_assert(NT >= 64 && (G == 1 || NW == 1), "a group is a wave or a workgroup");
+    __shared__ float sm[G][NW], ss[G][NW];
+    __shared__ float s_p[G][kEntries ? KM : 1], s_x[G][kEntries ? KM : 1];
+    __shared__ int s_id[G][kEntries ? KM : 1], s_next[G][kEntries ? KM : 1], s_head[G][kDz ? NT : 1];
+    __shared__ float s_tot[G][4];
+    const int gi = G == 1 ? 0 : threadIdx.x >> 6, u = G == 1 ? threadIdx.x : threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, w = G == 1 ? threadIdx.x >> 6 : 0;
+    auto sync = [&]() {
+        if (NW > 1)
+            __syncthreads();
+        else
+            __builtin_amdgcn_wave_barrier();  // (one wave: LDS operations are in order)
+    };
+    int64_t r = (int64_t)blockIdx.x * G + gi;
+    int slice = 0;
+    if (MODE == kPart || MODE == kJoin || MODE == kGrad) {
+        slice = (int)(r % a.slices);
+        r /= a.slices;
+    }
+    if (r >= a.rows) return;  // (a whole wave, only where groups are waves)
     const T *z = (const T *)a.z + r * a.ldz;
-    const float it = 1.0f / a.t;
-    float lse;
-    if (a.mode == 0) {
-        MS v = {-INFINITY, 0.0f};
-        for (int64_t j = tid; j < a.vocab; j += 256) {
-            const float x = D::up(z[j]) * it;
-            v = add(v, x == INFINITY ? NAN : x);
+    const float c = kLog2e / a.t;
+    // the slice's vectors [v0, v1) and places [j0, j1)
+    // -- the row's whole vectors; its last vocab % E elements are single, one to each of the last
+    // slice's first threads
+    const int nvec = (int)(a.vocab / E);
+    const int v0 = a.slices > 1 ? slice * kSliceVecs : 0;
+    const int v1 = a.slices > 1 ? min(nvec, v0 + kSliceVecs) : nvec;
+    const int t0 = slice == a.slices - 1 ? nvec * E : (int)a.vocab;  // (vocab: no single ones here)
+    const bool single = u < (int)a.vocab - t0;
+
+    // ------------------------------------------- the entries' loads first
+    int id[J];
+    float tv[J];
+    const bool first = kEntries && w == 0;
+    if (first) {
+#pragma unroll
+        for (int i = 0; i < J; ++i) {
+            const int j = i * 64 + lane;
+            int64_t k = -1;
+            tv[i] = -INFINITY;
+            if (j < a.top) {
+                k = a.ids64 ? ((const int64_t *)a.ids)[r * a.top + j] : ((const int32_t *)a.ids)[r * a.top + j];
+                tv[i] = a.tv[r * a.top + j];
+            }
+            id[i] = k < 0 ? -1 : k >= a.vocab ? INT32_MAX : (int)k;  // (vocab < INT32_MAX)
+        }
+    }
+    V x[NV ? NV : 1];
+    float m = -INFINITY, s = 0.0f;
+    if (kStats) {
+        if (NV) {
+            // (NV / 2 NT < whole vectors <= NV NT: only the later half can be missing; a missing one is
+            // read from the last one's place, which costs less than a branch round every load)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) x[i].load(z + (i < NV / 2 ? i * NT + u : min(i * NT + u, nvec - 1)) * E);
+        }
+    }
+    const float x1 = single ? D::up(z[t0 + u]) : -INFINITY;
+
+    // ------------------------------------------------------------ entries
+    // of the first wave: p, log2 p and the z they name; in LDS p, z, the id and the owner's list
+    float p[J], lp[J], xe[J];
+    float tot = 0.0f;
+    bool bad = false, any = false;
+    if (first) {
+        float L2;
+        float tm = -INFINITY;
+        if (a.teacher_lse) {
+            tm = 0.0f;
+            L2 = a.teacher_lse[r] * kLog2e;
+        } else {
+#pragma unroll
+            for (int i = 0; i < J; ++i)
+                if (id[i] >= 0) tm = fmaxf(tm, tv[i]);
+            tm = wave_max(tm);
+            if (tm == -INFINITY) tm = 0.0f;
+            float ts = 0.0f;
+#pragma unroll
+            for (int i = 0; i < J; ++i)
+                if (id[i] >= 0) ts += ex2((tv[i] - tm) * c);
+            ts = wave_sum(ts);
+            L2 = ts == 0.0f ? 0.0f : __builtin_amdgcn_logf(ts);
+        }
+        if (kDz) {
+#pragma unroll
+            for (int i = 0; i < NW; ++i) s_head[gi][i * 64 + lane] = -1;
+            __builtin_amdgcn_wave_barrier();
         }
 #pragma unroll
-        for (int s = 32; s >= 1; s >>= 1) v = join(v, {__shfl_xor(v.m, s), __shfl_xor(v.s, s)});
-        if (lane == 0) sm[w] = v.m, ss[w] = v.s;
-        __syncthreads();
-        v = {sm[0], ss[0]};
-        for (int i = 1; i < 4; ++i) v = join(v, {sm[i], ss[i]});
-        lse = v.m == -INFINITY && v.s == 0.0f ? -INFINITY : v.m + logf(v.s);
-        if (v.s != v.s) lse = NAN;
+        for (int i = 0; i < J; ++i) {
+            const int j = i * 64 + lane;
+            bad |= id[i] == INT32_MAX;
+            lp[i] = fmaf(tv[i] - tm, c, -L2);
+            p[i] = id[i] < 0 ? 0.0f : ex2(lp[i]);
+            if (a.teacher_lse && id[i] >= 0 && tv[i] != -INFINITY && p[i] != p[i]) bad = true;
+            any |= !(p[i] == 0.0f);
+            tot += p[i];
+            xe[i] = 0.0f;
+            const bool real = id[i] >= 0 && id[i] < a.vocab;
+            if (MODE == kJoin)
+                xe[i] = real ? a.xs[r * a.top + j] : 0.0f;
+            else if (real)
+                xe[i] = D::up(z[id[i]]);
+            if (kDz) {
+                s_p[gi][j] = p[i];
+                s_x[gi][j] = xe[i];
+                s_id[gi][j] = id[i];
+                const int v = id[i] / E;
+                if (real && (id[i] >= t0 || (v >= v0 && v < v1)))
+                    s_next[gi][j] = atomicExch(&s_head[gi][id[i] >= t0 ? id[i] - t0 : (v - v0) % NT], j);
+            }
+        }
+        tot = wave_sum(tot);
+        if (__any(bad)) tot = NAN;
+        any = __any(any) || tot != tot;
+    }
+    if (MODE == kPart && slice == 0 && w == 0) {
+        for (int j = lane; j < a.top; j += 64) {
+            const int64_t k = a.ids64 ? ((const int64_t *)a.ids)[r * a.top + j] : ((const int32_t *)a.ids)[r * a.top + j];
+            a.xs[r * a.top + j] = k >= 0 && k < a.vocab ? D::up(z[k]) : 0.0f;
+        }
+    }
+
+    // -------------------------------------------------- softmax statistics
+    if (kStats) {
+        m = x1;
+        if (NV) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (i >= NV / 2) x[i].mask(i * NT + u < nvec);
+                x[i].forget();
+                m = fmaxf(m, x[i].max());
+            }
+            m = wave_max(m);
+            const float mu = m == -INFINITY ? 0.0f : m;
+            s = single ? ex2((x1 - mu) * c) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                x[i].forget();
+                s += x[i].sum(mu, c);
+            }
+            s = wave_sum(s);
+        } else {
+            s = single ? ex2((x1 - (x1 == -INFINITY ? 0.0f : x1)) * c) : 0.0f;
+            // 4 vectors at a time: their maximum joins the running one first
+            for (int v = v0 + u; v < v1; v += 4 * NT) {
+                V y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (v + i * NT < v1) y[i].load(z + (v + i * NT) * E);
+                float n = m;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (v + i * NT < v1) n = fmaxf(n, y[i].max());
+                const float nu = n == -INFINITY ? 0.0f : n;
+                s *= m == -INFINITY ? (s != s ? s : 0.0f) : ex2((m - nu) * c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (v + i * NT < v1) s += y[i].sum(nu, c);
+                m = n;
+            }
+            const float wm = wave_max(m), wu = wm == -INFINITY ? 0.0f : wm;
+            s = wave_sum(s * (m == -INFINITY ? (s != s ? s : 0.0f) : ex2((m - wu) * c)));
+            m = wm;
+        }
+    }
+    if (NW > 1 && kStats && lane == 0) sm[gi][w] = m, ss[gi][w] = s;
+    if (NW > 1 && first && lane == 0) s_tot[gi][0] = tot, s_tot[gi][1] = any ? 1.0f : 0.0f;
+    sync();
+    if (NW > 1 && kEntries && !first) tot = s_tot[gi][0], any = s_tot[gi][1] != 0.0f;
+    auto join = [&](float m1, float s1) {
+        const float n = fmaxf(m, m1), nu = n == -INFINITY ? 0.0f : n;
+        s = (m == -INFINITY ? (s != s ? s : 0.0f) : s * ex2((m - nu) * c)) +
+            (m1 == -INFINITY ? (s1 != s1 ? s1 : 0.0f) : s1 * ex2((m1 - nu) * c));
+        m = n;
+    };
+    if (kStats && NW > 1) {
+        m = sm[gi][0], s = ss[gi][0];
+#pragma unroll
+        for (int i = 1; i < NW; ++i) join(sm[gi][i], ss[gi][i]);
+    }
+    if (MODE == kPart) {
+        if (u == 0) a.part[r * a.slices + slice] = make_float2(m, s);
+        return;
+    }
+    if (MODE == kJoin) {
+        const float2 *q = a.part + r * a.slices;
+        m = q[0].x, s = q[0].y;
+        for (int i = 1; i < a.slices; ++i) join(q[i].x, q[i].y);
+    }
+    float l2;
+    if (MODE == kGrad) {
+        const float *st = a.stats + r * 4;
+        m = st[0], l2 = st[1], tot = st[2];
+        any = tot != 0.0f;
     } else {
-        lse = a.stats[2 * r];
-        if (a.stats[2 * r + 1] != a.stats[2 * r + 1]) lse = NAN;
+        if (m == -INFINITY) m = 0.0f;
+        l2 = s == 0.0f ? 0.0f : __builtin_amdgcn_logf(s);
+        if (!any) tot = 0.0f;
+        if (any && l2 != l2) tot = NAN;
     }
-    // the teacher's entries
-    float tm = -INFINITY;
-    bool bad = false;
-    for (int j = tid; j < a.top; j += 256) {
-        const int64_t id = a.ids64 ? ((const int64_t *)a.ids)[r * a.top + j] : ((const int32_t *)a.ids)[r * a.top + j];
-        bad |= id >= a.vocab;
-        sid[j] = id;
-        sp[j] = id < 0 ? -INFINITY : a.tv[r * a.top + j] * it;
-    }
-    if (__syncthreads_or(bad)) lse = NAN;
-    MS tl = {-INFINITY, 0.0f};
-    if (a.teacher_lse)
-        tm = a.teacher_lse[r];
-    else {
-        for (int j = 0; j < a.top; ++j) tl = add(tl, sp[j]);
-        tm = tl.m + logf(tl.s);
-        if (tl.m == -INFINITY && tl.s == 0.0f) tm = -INFINITY;
-    }
-    __syncthreads();
-    float l = 0.0f, sum = 0.0f;
-    bool some = false;
-    for (int j = tid; j < a.top; j += 256) {
-        const int64_t id = sid[j];
-        const float lp = sp[j] - tm;
-        const float p = sp[j] == -INFINITY ? 0.0f : e2(lp);
-        sp[j] = p;
-        some |= id >= 0 && !(p == 0.0f);
-        const float x = id >= 0 && id < a.vocab ? D::up(z[id]) * it : 0.0f;
-        sx[j] = x;
-        if (!(p == 0.0f)) {
-            l += p * (lp - (x == -INFINITY ? x : x - lse));
-        }
-        sum += p;
-    }
+
+    // ---------------------------------------------------------------- loss
+    if (MODE != kGrad && first && slice == 0) {
+        float l = 0.0f;
 #pragma unroll
-    for (int s = 32; s >= 1; s >>= 1) l += __shfl_xor(l, s), sum += __shfl_xor(sum, s);
-    if (lane == 0) sm[w] = l, ss[w] = sum;
-    some = __syncthreads_or(some);
-    l = sm[0] + sm[1] + sm[2] + sm[3];
-    sum = ss[0] + ss[1] + ss[2] + ss[3];
-    if (lse != lse) l = sum = NAN, some = true;
-    if (!some) l = sum = 0.0f;
-    if (tid == 0) {
-        if (a.loss) a.loss[r] = a.t * a.t * l;
-        if (a.stats && a.mode == 0) a.stats[2 * r] = lse, a.stats[2 * r + 1] = sum;
+        for (int i = 0; i < J; ++i)
+            if (!(p[i] == 0.0f)) l += p[i] * (lp[i] - fmaf(xe[i] - m, c, -l2));
+        l = wave_sum(l);
+        if (tot != tot) l = NAN;
+        if (lane == 0) {
+            a.loss[r] = any ? a.t * a.t * kLn2 * l : 0.0f;
+            if (a.stats) *reinterpret_cast<f32x4 *>(a.stats + r * 4) = (f32x4){m, l2, tot, 0.0f};
+        }
     }
-    if (!a.dz) return;
-    T *dz = (T *)a.dz + r * a.ldd;
-    const float g = a.t * (a.row_scale ? a.row_scale[r * a.scale_stride] : 1.0f);
-    for (int64_t j = tid; j < a.vocab; j += 256) {
-        const float x = D::up(z[j]) * it;
-        const float q = x == -INFINITY && lse == lse ? 0.0f : e2(x - lse);
-        dz[j] = D::down(some ? g * (sum * q) : 0.0f);
-    }
-    if (!some || lse != lse) return;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();  // (the entries' places are written again below, after every store above has ended)
-    for (int j = tid; j < a.top; j += 256) {
-        const int64_t id = sid[j];
-        if (id < 0) continue;
-        float p = 0.0f;
-        bool first = true;
-        for (int i = 0; i < a.top; ++i)
-            if (sid[i] == id) p += sp[i], first &= i >= j;
-        if (!first) continue;
-        const float x = sx[j];  // (z's own place may hold dz by now)
-        const float q = x == -INFINITY ? 0.0f : e2(x - lse);
-        dz[id] = D::down(g * (sum * q - p));
+
+    // ------------------------------------------------------------ gradient
+    if (kDz) {
+        if (MODE == kJoin && !a.dz) return;
+        T *dz = (T *)a.dz + r * a.ldd;
+        const float g = a.t * (a.row_scale ? a.row_scale[r * a.scale_stride] : 1.0f), f = g * tot;
+        // (without an entry that counts every gradient is 0, not 0 times what may be NaN)
+        if (NV && MODE == kBoth) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                x[i].forget();
+                if (any)
+                    x[i].grad(m, c, l2, f);
+                else
+                    x[i] = V{};
+                if (i < NV / 2 || i * NT + u < nvec) x[i].store(dz + (i * NT + u) * E);
+            }
+        } else {
+            for (int v = v0 + u; v < v1; v += 4 * NT) {
+                V y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (v + i * NT < v1) y[i].load(z + (v + i * NT) * E);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (v + i * NT < v1) {
+                        if (any)
+                            y[i].grad(m, c, l2, f);
+                        else
+                            y[i] = V{};
+                        y[i].store(dz + (v + i * NT) * E);
+                    }
+            }
+        }
+        if (single) dz[t0 + u] = D::down(any ? f * ex2(fmaf(x1 - m, c, -l2)) : 0.0f);
+        if (!any || tot != tot) return;
+        // this thread's entries: of several with one id the first adds up all, in their order
+        for (int j = s_head[gi][u]; j >= 0; j = s_next[gi][j]) {
+            const int k = s_id[gi][j];
+            bool lead = true;
+            for (int i = s_head[gi][u]; i >= 0; i = s_next[gi][i]) lead &= !(s_id[gi][i] == k && i < j);
+            if (!lead) continue;
+            float sum = 0.0f;
+            for (int at = j; at < KM;) {
+                sum += s_p[gi][at];
+                int next = KM;
+                for (int i = s_head[gi][u]; i >= 0; i = s_next[gi][i])
+                    if (s_id[gi][i] == k && i > at && i < next) next = i;
+                at = next;
+            }
+            const float q = ex2(fmaf(s_x[gi][j] - m, c, -l2));
+            dz[k] = D::down(g * (tot * q - sum));
+        }
     }
 }
 
@@ -155,7 +405,7 @@ __global__ __launch_bounds__(1024) void k_distill_reduce(const float *loss, cons
     float l = 0.0f, c = 0.0f;
     for (int64_t r = tid; r < rows; r += 1024) {
         l += loss[r];
-        c += stats[2 * r + 1] == 0.0f ? 0.0f : 1.0f;
+        c += stats[4 * r + 2] == 0.0f ? 0.0f : 1.0f;
     }
 #pragma unroll
     for (int s = 32; s >= 1; s >>= 1) l += __shfl_xor(l, s), c += __shfl_xor(c, s);
@@ -169,17 +419,65 @@ __global__ __launch_bounds__(1024) void k_distill_reduce(const float *loss, cons
     out[1] = f;
 }
 
-static int run(const DistillArgs &a, int dtype, hipStream_t st) {
-    const dim3 g((unsigned)a.rows);
-    if (dtype == LIRA_DTYPE_F32)
-        hipLaunchKernelGGL((k_distill<F32>), g, dim3(256), 0, st, a);
-    else if (dtype == LIRA_DTYPE_BF16)
-        hipLaunchKernelGGL((k_distill<BF16>), g, dim3(256), 0, st, a);
-    else
-        hipLaunchKernelGGL((k_distill<F16>), g, dim3(256), 0, st, a);
+template <class D, int NT, int NV, int KM, Mode MODE>
+static int launch(const DistillArgs &a, hipStream_t st) {
+    constexpr int G = NT < 256 ? 256 / NT : 1;
+    const int64_t groups = a.rows * (MODE == kPart || MODE == kJoin || MODE == kGrad ? a.slices : 1);
+    if ((groups + G - 1) / G > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "distill: too many rows for one launch");
+    hipLaunchKernelGGL((k_distill<D, NT, NV, KM, MODE>), dim3((unsigned)((groups + G - 1) / G)), dim3(NT < 256 ? 256 : NT),
+                       0, st, a);
     LIRA_HIP_TRY(hipGetLastError());
     return LIRA_OK;
 }
+
+// slices of a row: enough workgroups for the 256 compute units where there are few long rows
+static int64_t distill_slices(int64_t rows, int64_t vecs) {
+    if (rows <= 0) return 1;
+    return std::max<int64_t>(1, std::min((vecs + kSliceVecs - 1) / kSliceVecs, rows >= 512 ? 1 : (vecs + kSliceVecs - 1) / kSliceVecs));
+}
+
+template <class D>
+static int run(DistillArgs a, bool grad_only, hipStream_t st) {
+    const int64_t vecs = a.vocab / Vec<D>::E;
+    const bool few = a.top <= 64;
+    if (grad_only) {
+        if (vecs <= 64 * 16 && few) return launch<D, 64, 0, 64, kGrad>(a, st);
+        a.slices = (int)std::max<int64_t>(1, (vecs + kSliceVecs - 1) / kSliceVecs);
+        return few ? launch<D, 256, 0, 64, kGrad>(a, st) : launch<D, 256, 0, kMaxTop, kGrad>(a, st);
+    }
+    if (a.slices > 1) {
+        if (int rc = launch<D, 256, 0, 64, kPart>(a, st)) return rc;
+        if (!a.dz) {
+            // (the loss alone: one group a row)
+            return few ? launch<D, 256, 0, 64, kJoin>(a, st) : launch<D, 256, 0, kMaxTop, kJoin>(a, st);
+        }
+        return few ? launch<D, 256, 0, 64, kJoin>(a, st) : launch<D, 256, 0, kMaxTop, kJoin>(a, st);
+    }
+    if (!a.dz) {
+        if (vecs <= 64 * 16 && few) return launch<D, 64, 0, 64, kLoss>(a, st);
+        return few ? launch<D, 256, 0, 64, kLoss>(a, st) : launch<D, 256, 0, kMaxTop, kLoss>(a, st);
+    }
+    if (!few) return launch<D, 256, 0, kMaxTop, kBoth>(a, st);
+    // the row in registers: a wave's up to 16 vectors a lane, then 256 and 1024 threads'
+    if (vecs < 1) return launch<D, 64, 0, 64, kBoth>(a, st);
+    if (vecs <= 64) return launch<D, 64, 1, 64, kBoth>(a, st);
+    if (vecs <= 64 * 2) return launch<D, 64, 2, 64, kBoth>(a, st);
+    if (vecs <= 64 * 4) return launch<D, 64, 4, 64, kBoth>(a, st);
+    if (vecs <= 64 * 8) return launch<D, 64, 8, 64, kBoth>(a, st);
+    if (vecs <= 64 * 16) return launch<D, 64, 16, 64, kBoth>(a, st);
+    if (vecs <= 256 * 8) return launch<D, 256, 8, 64, kBoth>(a, st);
+    if (vecs <= 256 * 16) return launch<D, 256, 16, 64, kBoth>(a, st);
+    if (vecs <= 1024 * 8) return launch<D, 1024, 8, 64, kBoth>(a, st);
+    if (vecs <= 1024 * 16) return launch<D, 1024, 16, 64, kBoth>(a, st);
+    return launch<D, 256, 0, 64, kBoth>(a, st);
+}
+static int run(const DistillArgs &a, int dtype, bool grad_only, hipStream_t st) {
+    if (dtype == LIRA_DTYPE_F32) return run<F32>(a, grad_only, st);
+    if (dtype == LIRA_DTYPE_BF16) return run<BF16>(a, grad_only, st);
+    return run<F16>(a, grad_only, st);
+}
+
+static int64_t vectors(int64_t vocab, int dtype) { return vocab / (dtype == LIRA_DTYPE_F32 ? 4 : 8); }
 
 }  // namespace lira
 
@@ -192,9 +490,11 @@ static int check_distill(const DistillArgs &a, int dtype, int ids_bits) {
     if (a.top < 1) return fail(LIRA_EINVAL, "top must be >= 1");
     if (a.top > kMaxTop) return fail(LIRA_EUNSUPPORTED, "top must be at most 1024");
     if (a.ldz < a.vocab || (a.dz && a.ldd < a.vocab)) return fail(LIRA_EINVAL, "row strides must be at least vocab");
-    if (!(a.t > 0.0f) || !(a.t < INFINITY)) return fail(LIRA_EINVAL, "temperature must be positive and finite");
+    if (!(a.t > 0.0f) || !(a.t < INFINITY) || !(kLog2e / a.t < INFINITY))
+        return fail(LIRA_EINVAL, "temperature must be positive and finite");
     if (a.row_scale && (a.scale_stride < 0 || a.scale_stride > 1))
         return fail(LIRA_EINVAL, "scale_stride must be 0 or 1");
+    if (a.vocab >= INT32_MAX) return fail(LIRA_EUNSUPPORTED, "vocab must be less than 2147483647");
     if (a.rows > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "too many rows for one launch");
     if (a.rows > 0 && (!a.z || !a.ids || !a.tv)) return fail(LIRA_EINVAL, "NULL buffer");
     return LIRA_OK;
@@ -202,16 +502,36 @@ static int check_distill(const DistillArgs &a, int dtype, int ids_bits) {
 
 extern "C" {
 
+int lira_distill_workspace_size(int64_t rows, int64_t vocab, int64_t top, int dtype, size_t *bytes) {
+    if (!bytes) return fail(LIRA_EINVAL, "NULL buffer");
+    if (dtype < LIRA_DTYPE_F32 || dtype > LIRA_DTYPE_F16) return fail(LIRA_EINVAL, "unknown dtype");
+    if (rows < 0 || vocab <= 0 || top < 1) return fail(LIRA_EINVAL, "bad shape");
+    const int64_t n = distill_slices(rows, vectors(vocab, dtype));
+    *bytes = n > 1 ? (size_t)(rows * (n * sizeof(float2) + top * sizeof(float))) : 0;
+    return LIRA_OK;
+}
+
 int lira_distill_topk(const void *z, int dtype, int64_t rows, int64_t vocab, int64_t ldz, const void *ids, int ids_bits,
                       const float *teacher, int64_t top, float temperature, const float *teacher_lse, float *loss,
                       float *stats, const float *row_scale, int64_t scale_stride, void *dz, int64_t ldd,
-                      void *stream) {
-    const DistillArgs a = {z, rows, vocab, ldz, ids, teacher, (int)(top < 0 ? 0 : top > INT32_MAX ? INT32_MAX : top),
-                           ids_bits == 64, teacher_lse, temperature, row_scale, scale_stride, loss, stats, dz, ldd, 0};
+                      void *workspace, size_t workspace_bytes, void *stream) {
+    DistillArgs a = {z, rows, vocab, ldz, ids, teacher, (int)(top < 0 ? 0 : top > INT32_MAX ? INT32_MAX : top),
+                     ids_bits == 64, teacher_lse, temperature, row_scale, scale_stride, loss, stats, dz, ldd, 1,
+                     nullptr, nullptr};
     if (int rc = check_distill(a, dtype, ids_bits)) return rc;
     if (rows == 0) return LIRA_OK;
     if (!loss) return fail(LIRA_EINVAL, "NULL buffer");
-    return run(a, dtype, (hipStream_t)stream);
+    if (((uintptr_t)stats & 15) != 0) return fail(LIRA_EINVAL, "stats must be 16-byte aligned");
+    size_t need = 0;
+    if (int rc = lira_distill_workspace_size(rows, vocab, top, dtype, &need)) return rc;
+    if (need) {
+        if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0)
+            return fail(LIRA_EINVAL, "workspace too small (lira_distill_workspace_size) or not 16-byte aligned");
+        a.slices = (int)distill_slices(rows, vectors(vocab, dtype));
+        a.part = (float2 *)workspace;
+        a.xs = (float *)(a.part + rows * a.slices);
+    }
+    return run(a, dtype, false, (hipStream_t)stream);
 }
 
 int lira_distill_topk_backward(const void *z, int dtype, int64_t rows, int64_t vocab, int64_t ldz, const void *ids,
@@ -220,11 +540,12 @@ int lira_distill_topk_backward(const void *z, int dtype, int64_t rows, int64_t v
                                int64_t scale_stride, void *dz, int64_t ldd, void *stream) {
     const DistillArgs a = {z, rows, vocab, ldz, ids, teacher, (int)(top < 0 ? 0 : top > INT32_MAX ? INT32_MAX : top),
                            ids_bits == 64, teacher_lse, temperature, row_scale, scale_stride, nullptr,
-                           const_cast<float *>(stats), dz, ldd, 1};
+                           const_cast<float *>(stats), dz, ldd, 1, nullptr, nullptr};
     if (int rc = check_distill(a, dtype, ids_bits)) return rc;
     if (rows == 0) return LIRA_OK;
     if (!stats || !dz) return fail(LIRA_EINVAL, "NULL buffer");
-    return run(a, dtype, (hipStream_t)stream);
+    if (((uintptr_t)stats & 15) != 0) return fail(LIRA_EINVAL, "stats must be 16-byte aligned");
+    return run(a, dtype, true, (hipStream_t)stream);
 }
 
 int lira_distill_reduce(const float *loss, const float *stats, int64_t rows, int mean, float *out, void *stream) {

@@ -21,16 +21,19 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 // element types of lira_hip.h's LIRA_DTYPE_*
 struct F32 {
     typedef float T;
+    static constexpr uint32_t kNegInf = 0xff800000u;
     static __device__ __forceinline__ float up(float v) { return v; }
     static __device__ __forceinline__ float down(float v) { return v; }
 };
 struct BF16 {
     typedef __bf16 T;
+    static constexpr uint32_t kNegInf = 0xff80u;
     static __device__ __forceinline__ float up(__bf16 v) { return (float)v; }
     static __device__ __forceinline__ __bf16 down(float v) { return (__bf16)v; }  // to nearest, ties to even
 };
 struct F16 {
     typedef _Float16 T;
+    static constexpr uint32_t kNegInf = 0xfc00u;
     static __device__ __forceinline__ float up(_Float16 v) { return (float)v; }
     static __device__ __forceinline__ _Float16 down(float v) { return (_Float16)v; }
 };

@@ -87,7 +87,8 @@ SIGNATURES = {
     "lira_mx4_linear": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _P, _I64, _I64, _F, _P, _INT, _P, _INT, _I64, _P,
                                _SZ, _P]),
     "lira_distill_topk": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _INT, _P, _I64, _F, _P, _P, _P, _P, _I64, _P, _I64,
-                                 _P]),
+                                 _P, _SZ, _P]),
+    "lira_distill_workspace_size": (_INT, [_I64, _I64, _I64, _INT, ctypes.POINTER(_SZ)]),
     "lira_distill_topk_backward": (_INT, [_P, _INT, _I64, _I64, _I64, _P, _INT, _P, _I64, _F, _P, _P, _P, _I64, _P,
                                           _I64, _P]),
     "lira_distill_reduce": (_INT, [_P, _P, _I64, _INT, _P, _P]),

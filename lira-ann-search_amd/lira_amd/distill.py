@@ -14,6 +14,8 @@ whose leaves no eager autograd graph still uses.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -69,15 +71,22 @@ def _head(z, ld, ids, tv, lse, t):
             tv.data_ptr(), ids.shape[1], t, _lib.ptr(lse))
 
 
+def _workspace(z, ids):
+    need = ctypes.c_size_t()
+    _lib.call("lira_distill_workspace_size", *z.shape, ids.shape[1], DTYPES[z.dtype], ctypes.byref(need))
+    return torch.empty(need.value, dtype=torch.uint8, device=z.device) if need.value else None
+
+
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, ids, tv, lse, t, reduction):
         z, ld = _rows(z)
         rows = z.shape[0]
         loss = torch.empty(rows, dtype=torch.float32, device=z.device)
-        stats = torch.empty((rows, 2), dtype=torch.float32, device=z.device)
+        stats = torch.empty((rows, 4), dtype=torch.float32, device=z.device)
+        ws = _workspace(z, ids)
         _lib.call("lira_distill_topk", *_head(z, ld, ids, tv, lse, t), loss.data_ptr(), stats.data_ptr(), None, 0, None,
-                  0, _lib.stream_ptr())
+                  0, _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_ptr())
         ctx.save_for_backward(z, ids, tv, lse, stats)
         ctx.t, ctx.factor = t, None
         if reduction == "none":
@@ -149,6 +158,8 @@ def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_
         w = None if row_weight is None else row_weight.detach().reshape(-1).to(torch.float32).contiguous()
         loss = torch.empty(rows, dtype=torch.float32, device=z.device)
         dz = torch.empty((rows, vocab), dtype=z.dtype, device=z.device) if grad_out is None else grad_out
+        ws = _workspace(z, ids)
         _lib.call("lira_distill_topk", *_head(z, ld, ids, tv, lse, float(temperature)), loss.data_ptr(), None,
-                  _lib.ptr(w), 1, dz.data_ptr(), vocab, _lib.stream_ptr())
+                  _lib.ptr(w), 1, dz.data_ptr(), vocab, _lib.ptr(ws), 0 if ws is None else ws.numel(),
+                  _lib.stream_ptr())
     return loss.view(lead), dz.view(logits.shape)

@@ -66,7 +66,7 @@ def check_grad(got, want, tol):
 
 
 CASES = [(1, 1, 1), (1, 7, 7), (3, 64, 5), (5, 257, 8), (64, 1000, 32), (17, 1024, 64), (2, 4097, 100), (33, 8192, 16),
-         (4, 32768, 64), (3, 50001, 10), (2, 131072, 64), (1, 300000, 1024), (700, 40, 3)]
+         (4, 32768, 64), (3, 50001, 10), (2, 131072, 64), (1, 300000, 1024), (700, 40, 3), (600, 7, 2), (520, 2000, 64), (515, 16391, 65), (513, 70001, 12), (513, 140000, 20)]
 
 
 @pytest.mark.parametrize("dtype", list(DT))

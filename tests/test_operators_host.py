@@ -72,7 +72,7 @@ def test_matmul_refusals_and_empty_calls():
 def test_distill_refusals(change, code, text):
     a = dict(z=A, dtype=0, rows=4, vocab=100, ldz=100, ids=A, bits=32, tv=A, top=5, t=1.0, out=A, stride=1, ldd=100) | change
     head = (a["z"], a["dtype"], a["rows"], a["vocab"], a["ldz"], a["ids"], a["bits"], a["tv"], a["top"], a["t"], None)
-    assert lib().lira_distill_topk(*head, a["out"], None, A, a["stride"], A, a["ldd"], None) == code
+    assert lib().lira_distill_topk(*head, a["out"], None, A, a["stride"], A, a["ldd"], A, 1 << 40, None) == code
     assert text in why()
     assert lib().lira_distill_topk_backward(*head, a["out"], A, a["stride"], A, a["ldd"], None) == code
     assert text in why()
@@ -80,8 +80,18 @@ def test_distill_refusals(change, code, text):
 
 def test_distill_empty_and_reduce():
     head = (None, 0, 0, 100, 100, None, 32, None, 5, 1.0, None)
-    assert lib().lira_distill_topk(*head, None, None, None, 0, None, 0, None) == 0
+    assert lib().lira_distill_topk(*head, None, None, None, 0, None, 0, None, 0, None) == 0
     assert lib().lira_distill_topk_backward(*head, None, None, 0, A, 100, None) == 0
+    few = (A, 1, 2, 100000, 100000, A, 32, A, 5, 1.0, None, A, None, None, 0, A, 100000)  # (split over the chip)
+    need = ctypes.c_size_t()
+    assert lib().lira_distill_workspace_size(2, 100000, 5, 1, ctypes.byref(need)) == 0 and need.value > 0
+    for ws, n in ((None, 1 << 40), (A, need.value - 1), (A + 4, 1 << 40)):
+        assert lib().lira_distill_topk(*few, ws, n, None) == -1 and "workspace" in why()
+    assert lib().lira_distill_workspace_size(2, 0, 5, 1, ctypes.byref(need)) == -1
+    assert lib().lira_distill_workspace_size(2, 10, 5, 7, ctypes.byref(need)) == -1
+    assert lib().lira_distill_workspace_size(2, 10, 5, 0, None) == -1
+    assert lib().lira_distill_topk(A, 0, 4, 10, 10, A, 32, A, 5, 1.0, None, A, A + 8, None, 0, A, 10, None, 0, None) == -1
+    assert "stats" in why()
     assert lib().lira_distill_reduce(A, A, -1, 0, A, None) == -1
     assert lib().lira_distill_reduce(None, A, 3, 0, A, None) == -1
     assert lib().lira_distill_reduce(A, A, 3, 0, None, None) == -1
