@@ -1,5 +1,6 @@
 // lira_mx4.hip -- microscaled 4-bit floats: packing, unpacking and the product on the matrix
 // cores (layout and format: lira_mx4.hpp).
+#include <algorithm>
 #include <string>
 
 #include "lira_internal.hpp"
@@ -21,13 +22,8 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(const typename D::T *__res
     const int64_t p = blockIdx.y;
     const bool live = row < n;
     float v[8];
-    load8<D, VEC>(x + (live ? row : 0) * ld, p * kPlane + lane * 8, k, v);
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, mag(v[i]));
-    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, false));  // lane ^ 1
-    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, false));  // lane ^ 2
-    const uint32_t s = scale_code(m);
+    load_run<D, VEC, 8>(x + (live ? row : 0) * ld, p * kPlane + lane * 8, k, v);
+    const uint32_t s = scale_code(quad_max(v));
     const uint32_t c = s == 255 ? 0u : to_codes(v, scale_operand(s));
     if (!live) return;
     const int64_t at = p * plane_rows + row;
@@ -35,23 +31,42 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(const typename D::T *__res
     if ((lane & 3) == 0) scales[at * 4 + (lane >> 2)] = (uint8_t)s;
 }
 
-template <class D>
+// A lane unpacks the E elements of one 16-byte store, so that a row's lanes write one run; a plane
+// takes 128 / E lanes.
+template <class D, bool VEC>
 __global__ __launch_bounds__(256) void k_mx4_dequantize(const uint8_t *__restrict__ codes,
                                                         const uint8_t *__restrict__ scales, int64_t plane_rows,
                                                         int64_t n, int64_t k, typename D::T *__restrict__ out,
                                                         int64_t ld) {
-    const int lane = threadIdx.x & 15;
-    const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    typedef typename D::T T;
+    constexpr int E = 16 / sizeof(T), L = kPlane / E;
+    const int lane = threadIdx.x % L;
+    const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
     const int64_t p = blockIdx.y;
     if (row >= n) return;
     const int64_t at = p * plane_rows + row;
-    const uint32_t c = *reinterpret_cast<const uint32_t *>(codes + at * 64 + lane * 4);
-    const uint32_t s = scales[at * 4 + (lane >> 2)];
-    const int64_t j = p * kPlane + lane * 8;
-    typename D::T *o = out + row * ld + j;
+    uint32_t c;
+    if (E == 8)
+        c = *reinterpret_cast<const uint32_t *>(codes + at * 64 + lane * 4);
+    else
+        c = *reinterpret_cast<const uint16_t *>(codes + at * 64 + lane * 2);
+    const uint32_t s = scales[at * 4 + lane * E / 32];
+    struct alignas(16) V {
+        T e[E];
+    } o;
+    float v[E];
+    from_codes<E>(c, s, v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (j + i < k) o[i] = D::down(from_code((c >> (4 * i)) & 15u, s));
+    for (int i = 0; i < E; ++i) o.e[i] = D::down(v[i]);
+    const int64_t j = p * kPlane + lane * E;
+    T *q = out + row * ld + j;
+    if (VEC && j + E <= k) {
+        *reinterpret_cast<V *>(q) = o;
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (j + i < k) q[i] = o.e[i];
+    }
 }
 
 // ------------------------------------------------------------------ product
@@ -81,12 +96,12 @@ __device__ __forceinline__ void finish(f32x4 (&acc)[N], f32x4 bias, const Epilog
                 acc[j][i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(acc[j][i] * -1.44269504088896340736f));
     }
 }
-// 4 columns of the bias, 0 where there is none
+// 4 columns of the bias, 0 where there is none (past the end the last one's: not stored)
 __device__ __forceinline__ f32x4 bias4(const Epilogue &e, int64_t col, int64_t n) {
     f32x4 b = {0, 0, 0, 0};
     if (e.bias) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = col + i < n ? e.bias[col + i] : 0.0f;
+        for (int i = 0; i < 4; ++i) b[i] = e.bias[min(col + i, n - 1)];
     }
     return b;
 }
@@ -94,7 +109,7 @@ template <class D>
 struct alignas(4 * sizeof(typename D::T)) Four {
     typename D::T v[4];
 };
-// 4 columns of one output row, rounded: in one store (aligned), or those of them that there are
+// 4 columns of one output row, rounded and stored (aligned)
 template <class D>
 __device__ __forceinline__ void store4(typename D::T *at, f32x4 y) {
     Four<D> o;
@@ -102,18 +117,32 @@ __device__ __forceinline__ void store4(typename D::T *at, f32x4 y) {
     for (int i = 0; i < 4; ++i) o.v[i] = D::down(y[i]);
     *reinterpret_cast<Four<D> *>(at) = o;
 }
+// the same at any alignment, or the first `left` of them
 template <class D>
-__device__ __forceinline__ void store_some(typename D::T *at, f32x4 y, int64_t left) {
+__device__ __forceinline__ void store_run(typename D::T *at, f32x4 y, int64_t left) {
+    Four<D> o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (i < left) at[i] = D::down(y[i]);
+    for (int i = 0; i < 4; ++i) o.v[i] = D::down(y[i]);
+    if (left >= 4) {
+        __builtin_memcpy(at, &o, sizeof(o));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < left) at[i] = o.v[i];
+    }
 }
 
 // LDS-DMA: lane l's `bytes` (16 or 4) at sbase + voff -> LDS byte lds + l * bytes.  Inline asm: hipcc
 // would wait for every DMA in flight before each LDS read (it cannot tell their places apart);
 // the pipeline below waits by count.  No register is written but M0, which is restored.
+__device__ __forceinline__ const uint8_t *scalar(const uint8_t *p) {  // (the same in every lane)
+    const uint64_t v = (uint64_t)p;
+    return (const uint8_t *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 |
+                             (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
 __device__ __forceinline__ void dma16(uint32_t lds, const uint8_t *sbase, uint32_t voff) {
     uint32_t keep;
+    sbase = scalar(sbase);
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep)
                  : "s"(lds), "v"(voff), "s"(sbase)
@@ -121,6 +150,7 @@ __device__ __forceinline__ void dma16(uint32_t lds, const uint8_t *sbase, uint32
 }
 __device__ __forceinline__ void dma4(uint32_t lds, const uint8_t *sbase, uint32_t voff) {
     uint32_t keep;
+    sbase = scalar(sbase);
     asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %2, %3\n\ts_mov_b32 m0, %0"
                  : "=&s"(keep)
                  : "s"(lds), "v"(voff), "s"(sbase)
@@ -130,9 +160,10 @@ template <int N>
 __device__ __forceinline__ void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-// a row's 4 blocks of a plane sit in LDS at 16-byte slots (block ^ turn(row)): the 16 rows that a
-// fragment read touches at one block then fall on different banks
-__device__ __forceinline__ uint32_t turn(uint32_t row) { return ((row >> 2) & 1u) | ((((row >> 1) ^ (row >> 3)) & 1u) << 1); }
+// A row's 4 blocks of a plane sit in LDS at 16-byte places (block ^ turn(row)).  An LDS read of 16 bytes a lane
+// takes 16 lanes at a time over the 64 banks, lanes 0-3, 12-15, 20-27 first, then 4-11, 16-19,
+// 28-31, and the upper half alike (measured): with this turn no two of them are on one bank.
+__device__ __forceinline__ uint32_t turn(uint32_t row) { return (row >> 1) & 3u; }
 
 struct Product {
     const uint8_t *ac, *as;  // rows of the output (m)
@@ -143,20 +174,34 @@ struct Product {
     void *out;
 };
 
-// The tile kernel: TN columns x TM rows of the output, WN x WM waves of 64 lanes.  Planes of 128
-// elements stream through kSlots LDS slots by LDS-DMA; a wave reads plane s + 1's fragments while
-// the matrix instructions of plane s run, so both come from registers.
-template <int TN, int TM, int WN, int WM, class D>
+// W's fragment x the rows' fragment + acc: lane l holds block l / 16 of row l % 16.  (The 32 x 32 x 64 form
+// has 1.4 times the rate by itself, 7.8 against 5.7 PFLOP/s, but the kernel around it is bound by its
+// loads: 8192^3 0.30 ms with it, 0.29 so.)
+__device__ __forceinline__ i32x8 wide(i32x4 v) { return (i32x8){v.x, v.y, v.z, v.w, 0, 0, 0, 0}; }
+__device__ __forceinline__ f32x4 mfma(i32x4 b, int sb, i32x4 a, int sa, f32x4 acc) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(b), wide(a), acc, 4, 4, 0, sb, 0, sa);
+}
+
+// The tile kernel: TN columns x TM rows of the output by WN x WM x WK waves.  Planes of 128 elements
+// stream through SLOTS LDS slots of PS planes by LDS-DMA, all slots but one in flight.  The WN x WM
+// waves split the tile; where a tile is small, WK such sets of waves split a slot's planes (there
+// is one barrier a slot, and a set's LDS reads and matrix instructions wait for each
+// other: with more sets, less of that is left bare) and join their sums in LDS in a fixed order.
+template <int TN, int TM, int WN, int WM, int WK, int SLOTS, int PS>
 struct Tile {
-    static constexpr int NW = WN * WM, FN = TN / WN / 16, FM = TM / WM / 16;
-    static constexpr int kSlots = 4;
-    static constexpr int kSlotBytes = (TN + TM) * 68;
-    static constexpr int kCodeLoads = (TN + TM) / 16 / NW;                        // per wave and plane
-    static constexpr int kScaleJobs = (TN + 63) / 64 + (TM + 63) / 64;            // of 64 rows
-    static constexpr int kScaleLoads = (kScaleJobs + NW - 1) / NW;                // (some waves repeat one)
+    static constexpr int NW = WN * WM * WK, FN = TN / WN / 16, FM = TM / WM / 16;
+    static constexpr int kCodeJobs = (TN + TM) / 16;                               // of 16 rows, a plane
+    static constexpr int kNb = (TN + 63) / 64, kScaleJobs = kNb + (TM + 63) / 64;  // of up to 64 rows, a plane
+    // per wave and slot (every wave makes the same number, so that it can wait by count: one without
+    // a job of its own repeats another's)
+    static constexpr int kCodeLoads = (kCodeJobs * PS + NW - 1) / NW, kScaleLoads = (kScaleJobs * PS + NW - 1) / NW;
     static constexpr int kLoads = kCodeLoads + kScaleLoads;
-    static constexpr int kBytes = kSlots * kSlotBytes;
-    static_assert((TN + TM) / 16 % NW == 0, "whole loads per wave");
+    // a plane of a slot: the codes of both sides, then their scales, 256 bytes a job (a side under 64 rows
+    // fills its job's lanes by repeating its last row)
+    static constexpr int kScaleAt = (TN + TM) * 64, kPlaneBytes = kScaleAt + kScaleJobs * 256;
+    static constexpr int kBytes = SLOTS * PS * kPlaneBytes;
+    static_assert(PS % WK == 0, "the sets split a slot's planes evenly");
+    static_assert(WK == 1 || NW * FN * FM * 1024 <= kBytes, "the sets' sums fit the slots");
 
     struct Frags {
         i32x4 b[FN], a[FM];
@@ -164,13 +209,13 @@ struct Tile {
     };
 };
 
-template <int TN, int TM, int WN, int WM, class D>
-__global__ __launch_bounds__(WN *WM * 64) void k_mx4_tile(Product P, int tiles_n, int tiles_m) {
-    typedef Tile<TN, TM, WN, WM, D> C;
+template <int TN, int TM, int WN, int WM, int WK, int SLOTS, int PS, class D>
+__global__ __launch_bounds__(WN *WM *WK * 64) void k_mx4_tile(Product P, int tiles_n, int tiles_m) {
+    typedef Tile<TN, TM, WN, WM, WK, SLOTS, PS> C;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wn = w % WN, wm = w / WN;
+    const int wn = w % WN, wm = w / WN % WM, wk = w / (WN * WM);
 
     // Workgroups go to the 8 XCDs in turn: each XCD takes a run of tiles of its own, 8 tiles of rows
     // by as many of columns, so that the tiles in flight on it share their operands in its L2.
@@ -185,46 +230,46 @@ __global__ __launch_bounds__(WN *WM * 64) void k_mx4_tile(Product P, int tiles_n
     const int64_t m0 = (band * 8 + in % hb) * TM, n0 = in / hb * TN;
 
     const uint32_t lds = (uint32_t)(uintptr_t)smem;
-    // this wave's loads of a plane: 16 rows each, codes first
     const uint8_t *cb = P.bc + n0 * 64, *ca = P.ac + m0 * 64, *sb = P.bs + n0 * 4, *sa = P.as + m0 * 4;
     const int64_t bstep = P.b_rows * 64, astep = P.a_rows * 64;
     const uint32_t nlast = (uint32_t)(min(P.n - n0, (int64_t)TN) - 1), mlast = (uint32_t)(min(P.m - m0, (int64_t)TM) - 1);
     uint32_t off[C::kCodeLoads], soff[C::kScaleLoads];
 #pragma unroll
     for (int i = 0; i < C::kCodeLoads; ++i) {
-        const uint32_t row = (uint32_t)((i * C::NW + w) * 16 + (lane >> 2));  // of the TN + TM rows
-        const bool bside = (i * C::NW + w) * 16 < TN;
-        const uint32_t rr = bside ? min(row, nlast) : min(row - TN, mlast);
+        const int first = (i * C::NW + w) % (C::kCodeJobs * PS) % C::kCodeJobs * 16;
+        const uint32_t row = (uint32_t)(first + (lane >> 2));  // of the TN + TM rows
+        const uint32_t rr = first < TN ? min(row, nlast) : min(row - TN, mlast);
         off[i] = rr * 64 + (((uint32_t)lane & 3u) ^ turn(row)) * 16;
     }
 #pragma unroll
     for (int i = 0; i < C::kScaleLoads; ++i) {
-        const int job = (i * C::NW + w) % C::kScaleJobs;
-        constexpr int nb = (TN + 63) / 64;
-        soff[i] = job < nb ? min((uint32_t)(job * 64 + lane), nlast) * 4 : min((uint32_t)((job - nb) * 64 + lane), mlast) * 4;
+        const int job = (i * C::NW + w) % (C::kScaleJobs * PS) % C::kScaleJobs;
+        soff[i] = job < C::kNb ? min((uint32_t)(job * 64 + lane), nlast) * 4
+                               : min((uint32_t)((job - C::kNb) * 64 + lane), mlast) * 4;
     }
-    auto fetch = [&](int p, int slot) {
-        const uint32_t base = lds + slot * C::kSlotBytes;
-        const uint8_t *pb = cb + p * bstep, *pa = ca + p * astep;
+    const int planes = P.planes, steps = (planes + PS - 1) / PS;
+    auto fetch = [&](int s) {
+        const uint32_t base = lds + s % SLOTS * (PS * C::kPlaneBytes);
 #pragma unroll
         for (int i = 0; i < C::kCodeLoads; ++i) {
-            const int rows = (i * C::NW + w) * 16;
-            dma16(base + rows * 64, rows < TN ? pb : pa, off[i]);
+            const int job = (i * C::NW + w) % (C::kCodeJobs * PS), q = job / C::kCodeJobs, rows = job % C::kCodeJobs * 16;
+            const int64_t p = PS == 1 ? s : min(s * PS + q, planes - 1);  // (past the end: any plane, not multiplied)
+            dma16(base + q * C::kPlaneBytes + rows * 64, rows < TN ? cb + p * bstep : ca + p * astep, off[i]);
         }
-        const uint8_t *qb = sb + p * (bstep >> 4), *qa = sa + p * (astep >> 4);
 #pragma unroll
         for (int i = 0; i < C::kScaleLoads; ++i) {
-            const int job = (i * C::NW + w) % C::kScaleJobs;
-            constexpr int nb = (TN + 63) / 64;
-            dma4(base + (TN + TM) * 64 + (job < nb ? job * 256 : TN * 4 + (job - nb) * 256), job < nb ? qb : qa, soff[i]);
+            const int all = (i * C::NW + w) % (C::kScaleJobs * PS), q = all / C::kScaleJobs, job = all % C::kScaleJobs;
+            const int64_t p = PS == 1 ? s : min(s * PS + q, planes - 1);
+            dma4(base + q * C::kPlaneBytes + C::kScaleAt + job * 256,
+                 job < C::kNb ? sb + p * (bstep >> 4) : sa + p * (astep >> 4), soff[i]);
         }
     };
-    const uint32_t frag_row = (uint32_t)r * 64 + (((uint32_t)g ^ turn((uint32_t)r)) * 16);
-    auto read = [&](int slot, typename C::Frags &f) {
-        const uint8_t *base = smem + slot * C::kSlotBytes;
-        const uint8_t *fb = base + wn * (TN / WN) * 64 + frag_row, *fa = base + (TN + wm * (TM / WM)) * 64 + frag_row;
-        const uint8_t *zb = base + (TN + TM) * 64 + wn * (TN / WN) * 4 + r * 4 + g;
-        const uint8_t *za = base + (TN + TM) * 64 + TN * 4 + wm * (TM / WM) * 4 + r * 4 + g;
+    const uint32_t turned = ((uint32_t)g ^ turn((uint32_t)r)) * 16;
+    auto read = [&](int at, typename C::Frags &f) {
+        const uint8_t *base = smem + at * C::kPlaneBytes;
+        const uint8_t *fb = base + (wn * (TN / WN) + r) * 64 + turned, *fa = base + (TN + wm * (TM / WM) + r) * 64 + turned;
+        const uint8_t *zb = base + C::kScaleAt + (wn * (TN / WN) + r) * 4 + g;
+        const uint8_t *za = base + C::kScaleAt + C::kNb * 256 + (wm * (TM / WM) + r) * 4 + g;
 #pragma unroll
         for (int i = 0; i < C::FN; ++i) f.b[i] = *reinterpret_cast<const i32x4 *>(fb + i * 1024), f.sb[i] = zb[i * 64];
 #pragma unroll
@@ -239,50 +284,221 @@ __global__ __launch_bounds__(WN *WM * 64) void k_mx4_tile(Product P, int tiles_n
 #pragma unroll
         for (int j = 0; j < C::FM; ++j)
 #pragma unroll
-            for (int i = 0; i < C::FN; ++i) {
-                const i32x8 B = {f.b[i].x, f.b[i].y, f.b[i].z, f.b[i].w, 0, 0, 0, 0};
-                const i32x8 A = {f.a[j].x, f.a[j].y, f.a[j].z, f.a[j].w, 0, 0, 0, 0};
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(B, A, acc[i][j], 4, 4, 0, f.sb[i], 0, f.sa[j]);
-            }
+            for (int i = 0; i < C::FN; ++i) acc[i][j] = mfma(f.b[i], f.sb[i], f.a[j], f.sa[j], acc[i][j]);
     };
-    const int planes = P.planes;
-    // before plane s is read: its loads have landed (those of the two planes after it may be in
-    // flight), and every wave has read plane s - 1, whose slot takes plane s + 3
+    // before slot s is read: its loads have landed (those of the slots after it may be in flight),
+    // and every wave has read slot s - 1, whose place takes the next one
+    constexpr int kAhead = SLOTS - 1;
+    static_assert((kAhead - 1) * C::kLoads <= 63, "vmcnt counts to 63");
     auto arrive = [&](int s) {
-        if (s + 2 < planes)
+        const int after = steps - 1 - s;
+        if (after >= kAhead - 1)
+            wait_vm<(kAhead - 1) * C::kLoads>();
+        else if (kAhead > 4 && after >= 3)
+            wait_vm<3 * C::kLoads>();
+        else if (kAhead > 3 && after == 2)
             wait_vm<2 * C::kLoads>();
-        else if (s + 1 < planes)
+        else if (kAhead > 2 && after == 1)
             wait_vm<C::kLoads>();
         else
             wait_vm<0>();
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (s + 3 < planes) fetch(s + 3, (s + 3) % C::kSlots);
+        if (s + kAhead < steps) fetch(s + kAhead);
     };
-    for (int p = 0; p < 3 && p < planes; ++p) fetch(p, p);
-    for (int s = 0; s < planes; ++s) {
+    for (int s = 0; s < kAhead && s < steps; ++s) fetch(s);
+    for (int s = 0; s < steps; ++s) {
         arrive(s);
-        typename C::Frags f;
-        read(s % C::kSlots, f);
-        multiply(f);
+        typename C::Frags f[PS / WK];
+#pragma unroll
+        for (int q = 0; q < PS / WK; ++q) read(s % SLOTS * PS + q * WK + wk, f[q]);
+#pragma unroll
+        for (int q = 0; q < PS / WK; ++q)
+            if (PS == 1 || s * PS + q * WK + wk < planes) multiply(f[q]);
+    }
+    if (WK > 1) {
+        // set k's sums at [fragment][k]; the sets share the fragments out among themselves
+        __syncthreads();  // (every slot has been read)
+        f32x4 *red = reinterpret_cast<f32x4 *>(smem) + (w % (WN * WM)) * (C::FN * C::FM * WK * 64) + lane;
+#pragma unroll
+        for (int i = 0; i < C::FN; ++i)
+#pragma unroll
+            for (int j = 0; j < C::FM; ++j) red[((i * C::FM + j) * WK + wk) * 64] = acc[i][j];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < C::FN; ++i)
+#pragma unroll
+            for (int j = 0; j < C::FM; ++j) {
+                if ((i * C::FM + j) % WK != wk) continue;
+                f32x4 y = red[(i * C::FM + j) * WK * 64];
+#pragma unroll
+                for (int k = 1; k < WK; ++k) y += red[((i * C::FM + j) * WK + k) * 64];
+                acc[i][j] = y;
+            }
     }
 
     // lane l of a fragment: output row l % 16, columns 4 (l / 16) ..
     typedef typename D::T T;
-    const int64_t row0 = m0 + wm * (TM / WM) + r, col0 = n0 + wn * (TN / WN) + g * 4;
-    T *out = (T *)P.out + row0 * P.ldo + col0;
-    const bool whole = m0 + TM <= P.m && n0 + TN <= P.n && ((uintptr_t)P.out & (sizeof(Four<D>) - 1)) == 0 && P.ldo % 4 == 0;
+    constexpr int TNw = TN / WN, TMw = TM / WM;
+    const int64_t row0 = m0 + wm * TMw, col0 = n0 + wn * TNw;
+    if (WK > 1) {
 #pragma unroll
-    for (int i = 0; i < C::FN; ++i) {
-        finish(acc[i], bias4(P.ep, col0 + i * 16, P.n), P.ep);
-        if (whole) {
+        for (int i = 0; i < C::FN; ++i) {
+            const int64_t col = col0 + i * 16 + g * 4;
+            finish(acc[i], bias4(P.ep, col, P.n), P.ep);
 #pragma unroll
-            for (int j = 0; j < C::FM; ++j) store4<D>(out + j * 16 * P.ldo + i * 16, acc[i][j]);
-        } else {
+            for (int j = 0; j < C::FM; ++j) {
+                const int64_t row = row0 + j * 16 + r;
+                if ((i * C::FM + j) % WK != wk || row >= P.m) continue;
+                store_run<D>((T *)P.out + row * P.ldo + col, acc[i][j], P.n - col);
+            }
+        }
+        return;
+    }
+    // 16 rows at a time through LDS, a region a wave, so that a wave writes whole runs of a row: straight from
+    // the fragments a bf16 store is runs of 32 bytes, 16 rows apart (8192^3 with them 0.35 ms, so 0.29)
+    constexpr int E = 16 / sizeof(T), kRow = TNw + E, kUnits = 16 * TNw / E;
+    static_assert(C::NW * 16 * kRow * (int)sizeof(T) <= C::kBytes, "the waves' regions fit the slots");
+    __syncthreads();  // (every slot has been read)
+    T *stage = reinterpret_cast<T *>(smem) + w * (16 * kRow);
 #pragma unroll
-            for (int j = 0; j < C::FM; ++j)
-                if (row0 + j * 16 < P.m) store_some<D>(out + j * 16 * P.ldo + i * 16, acc[i][j], P.n - (col0 + i * 16));
+    for (int i = 0; i < C::FN; ++i) finish(acc[i], bias4(P.ep, col0 + i * 16 + g * 4, P.n), P.ep);
+#pragma unroll
+    for (int j = 0; j < C::FM; ++j) {
+#pragma unroll
+        for (int i = 0; i < C::FN; ++i) store4<D>(stage + r * kRow + i * 16 + g * 4, acc[i][j]);
+        __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are in order)
+#pragma unroll
+        for (int u = 0; u < (kUnits + 63) / 64; ++u) {
+            const int at = u * 64 + lane, rr = at / (TNw / E), c = at % (TNw / E) * E;
+            const int64_t row = row0 + j * 16 + rr, col = col0 + c;
+            if (at < kUnits && row < P.m && col < P.n) {
+                struct alignas(16) V {
+                    T e[E];
+                };
+                const V v = *reinterpret_cast<const V *>(stage + rr * kRow + c);
+                T *o = (T *)P.out + row * P.ldo + col;
+                if (col + E <= P.n) {
+                    __builtin_memcpy(o, &v, 16);  // (at any alignment)
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (col + e < P.n) o[e] = v.e[e];
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The few-rows kernel: 16 NB columns of the output x up to 16 rows, a stream over W.  No operand is
+// shared between waves, so W goes straight to registers: a wave's load of a fragment is 1 KiB in a row.
+// KS waves of a workgroup split the planes and join their sums in LDS in a fixed order.  KS = 1, where
+// there are few planes: four waves, each of its own columns, and workgroups that go on to the next
+// columns, whose first plane is on its way while the last one is finished.  FUSED: the rows of x are
+// packed here, 32 elements a thread, while the first planes of W are on their way; else they come
+// packed and are read from the cache.
+struct Rows {
+    const void *x;  // FUSED: (m, k), row stride ldx
+    int64_t k, ldx;
+};
+template <class X, class D, int NB, int KS, bool FUSED, bool VEC>
+__global__ __launch_bounds__(KS == 1 ? 256 : KS * 64, 4) void k_mx4_rows(Product P, Rows R) {
+    constexpr int U = KS == 1 ? 1 : FUSED ? 3 : 4;  // planes in flight
+    constexpr int NT = KS == 1 ? 256 : KS * 64;
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int planes = P.planes, first = KS == 1 ? 0 : w, m = (int)P.m;
+    const int64_t groups = (P.n + 16 * NB - 1) / (16 * NB), step = KS == 1 ? (int64_t)gridDim.x * 4 : groups;
+    int64_t group = KS == 1 ? (int64_t)blockIdx.x * 4 + w : blockIdx.x;
+    const int64_t bplane = P.b_rows * 64, aplane = P.a_rows * 64;
+    const int ao = min(r, m - 1);  // (rows past the end read the last one's place)
+    struct Step {
+        i32x4 b[NB], a;
+        int sb[NB], sa;
+    } f[U];
+    const int stride = FUSED ? planes * 64 + 16 : 0;  // of a packed row in LDS (its banks turn by 4)
+    uint8_t *xs = smem + (FUSED ? m * stride : 0);
+    auto load = [&](Step &q, int64_t grp, int p) {
+        const int64_t row = grp * (16 * NB);
+        const uint8_t *c = P.bc + p * bplane + row * 64, *s = P.bs + p * (bplane >> 4) + row * 4;
+        const int last = (int)min(P.n - row, (int64_t)16 * NB) - 1;  // (rows past the end read the last one's place)
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const uint32_t at = (uint32_t)min(i * 16 + r, last) * 4 + g;
+            q.b[i] = __builtin_nontemporal_load(reinterpret_cast<const i32x4 *>(c + at * 16));
+            q.sb[i] = s[at];
+        }
+        if (!FUSED) {
+            q.a = *reinterpret_cast<const i32x4 *>(P.ac + p * aplane + ao * 64 + g * 16);
+            q.sa = P.as[p * (aplane >> 4) + ao * 4 + g];
+        }
+    };
+    if (KS > 1 || group < groups) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) load(f[u], group, min(first + u * KS, planes - 1));
+    }
+    if (FUSED) {
+        // 8 elements a thread, the blocks' largest by DPP as in k_mx4_quantize
+        const int runs = planes * 16;
+        for (int b = threadIdx.x; b < m * runs; b += NT) {
+            const int row = m == 1 ? 0 : b / runs, run = b - row * runs;
+            float v[8];
+            load_run<X, VEC, 8>((const typename X::T *)R.x + row * R.ldx, run * 8, R.k, v);
+            const uint32_t s = scale_code(quad_max(v));
+            *reinterpret_cast<uint32_t *>(smem + row * stride + run * 4) = s == 255 ? 0u : to_codes(v, scale_operand(s));
+            if ((run & 3) == 0) xs[row * planes * 4 + (run >> 2)] = (uint8_t)s;
+        }
+        __syncthreads();
+    }
+    auto store = [&](f32x4 y, f32x4 bias, int64_t col) {
+        if (r >= m || col >= P.n) return;
+        f32x4 t[1] = {y};
+        finish(t, bias, P.ep);
+        store_run<D>((typename D::T *)P.out + r * P.ldo + col, t[0], P.n - col);
+    };
+    for (; group < groups; group += step) {
+        f32x4 acc[NB], bias[NB];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            acc[i] = (f32x4){0, 0, 0, 0};
+            if (KS == 1) bias[i] = bias4(P.ep, group * (16 * NB) + i * 16 + g * 4, P.n);
+        }
+        for (int p = first; p < planes; p += U * KS) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (p + u * KS >= planes) break;  // (the whole wave)
+                if (FUSED) {
+                    f[u].a = *reinterpret_cast<const i32x4 *>(smem + ao * stride + (p + u * KS) * 64 + g * 16);
+                    f[u].sa = xs[ao * planes * 4 + (p + u * KS) * 4 + g];
+                }
+#pragma unroll
+                for (int i = 0; i < NB; ++i) acc[i] = mfma(f[u].b[i], f[u].sb[i], f[u].a, f[u].sa, acc[i]);
+                const int next = p + (U + u) * KS;
+                if (next < planes)
+                    load(f[u], group, next);
+                else if (KS == 1 && group + step < groups)
+                    load(f[u], group + step, 0);
+            }
+        }
+        if (KS == 1) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) store(acc[i], bias[i], group * (16 * NB) + i * 16 + g * 4);
+            continue;
+        }
+        __syncthreads();  // (the packed rows are no longer read)
+        f32x4 *red = reinterpret_cast<f32x4 *>(smem);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) red[(i * KS + w) * 64 + lane] = acc[i];
+        __syncthreads();
+        for (int t = w; t < NB; t += KS) {
+            f32x4 y = red[t * KS * 64 + lane];
+#pragma unroll
+            for (int q = 1; q < KS; ++q) y += red[(t * KS + q) * 64 + lane];
+            const int64_t col = group * (16 * NB) + t * 16 + g * 4;
+            store(y, bias4(P.ep, col, P.n), col);
         }
     }
 }
@@ -319,26 +535,90 @@ static int quantize(const void *x, int64_t n, int64_t k, int64_t ld, uint8_t *co
     return LIRA_OK;
 }
 
-template <int TN, int TM, int WN, int WM, class D>
+template <class D>
+static int dequantize(const uint8_t *codes, const uint8_t *scales, int64_t plane_rows, int64_t n, int64_t k, void *out,
+                      int64_t ld, hipStream_t st) {
+    typedef typename D::T T;
+    constexpr int R = 256 / (kPlane / (16 / (int)sizeof(T)));  // rows of a workgroup
+    const bool vec = ((uintptr_t)out & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
+    const dim3 g((unsigned)((n + R - 1) / R), (unsigned)planes_of(k));
+    if (vec)
+        hipLaunchKernelGGL((k_mx4_dequantize<D, true>), g, dim3(256), 0, st, codes, scales, plane_rows, n, k, (T *)out, ld);
+    else
+        hipLaunchKernelGGL((k_mx4_dequantize<D, false>), g, dim3(256), 0, st, codes, scales, plane_rows, n, k, (T *)out, ld);
+    LIRA_HIP_TRY(hipGetLastError());
+    return LIRA_OK;
+}
+
+template <int TN, int TM, int WN, int WM, int WK, int SLOTS, int PS, class D>
 static int launch_tile(const Product &p, hipStream_t st) {
-    typedef Tile<TN, TM, WN, WM, D> C;
+    typedef Tile<TN, TM, WN, WM, WK, SLOTS, PS> C;
+    static_assert(C::kBytes <= 163840, "160 KB of LDS");
     static std::atomic<uint64_t> latch{0};
-    const void *fn = (const void *)&k_mx4_tile<TN, TM, WN, WM, D>;
+    const void *fn = (const void *)&k_mx4_tile<TN, TM, WN, WM, WK, SLOTS, PS, D>;
     LIRA_HIP_TRY(set_smem_attr_once(latch, fn, C::kBytes));
     const int64_t tn = (p.n + TN - 1) / TN, tm = (p.m + TM - 1) / TM;
     if (tn * tm > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "product: too many tiles for one launch");
-    hipLaunchKernelGGL((k_mx4_tile<TN, TM, WN, WM, D>), dim3((unsigned)(tn * tm)), dim3(WN * WM * 64), C::kBytes, st, p,
+    hipLaunchKernelGGL((k_mx4_tile<TN, TM, WN, WM, WK, SLOTS, PS, D>), dim3((unsigned)(tn * tm)), dim3(C::NW * 64), C::kBytes, st, p,
                        (int)tn, (int)tm);
     LIRA_HIP_TRY(hipGetLastError());
     return LIRA_OK;
 }
 
+template <class X, class D, int NB, int KS, bool FUSED, bool VEC>
+static int launch_rows(const Product &p, const Rows &r, hipStream_t st) {
+    static std::atomic<uint64_t> latch{0};
+    const void *fn = (const void *)&k_mx4_rows<X, D, NB, KS, FUSED, VEC>;
+    const int bytes = std::max(KS == 1 ? 0 : KS * NB * 1024, FUSED ? (int)p.m * (p.planes * 68 + 16) : 0);
+    LIRA_HIP_TRY(set_smem_attr_once(latch, fn, 65536));
+    const int64_t groups = (p.n + 16 * NB - 1) / (16 * NB);
+    // (KS = 1: as many workgroups of 4 waves as the 256 compute units hold, 4 waves a SIMD)
+    const int64_t blocks = KS == 1 ? std::min<int64_t>((groups + 3) / 4, 256 * 6) : groups;
+    hipLaunchKernelGGL((k_mx4_rows<X, D, NB, KS, FUSED, VEC>), dim3((unsigned)blocks), dim3(KS == 1 ? 256 : KS * 64), bytes, st,
+                       p, r);
+    LIRA_HIP_TRY(hipGetLastError());
+    return LIRA_OK;
+}
+// Rows that the product packs by itself: so few that every workgroup may do it again.
+static constexpr int64_t kFusedMax = 4;
+static bool fused_rows(int64_t m, int64_t k) { return m <= kFusedMax && m * (planes_of(k) * 68 + 16) <= 49152; }
+
+template <class X, class D>
+static int linear_rows(const Product &p, const Rows &r, hipStream_t st) {
+    const bool vec = ((uintptr_t)r.x & 15) == 0 && (r.ldx * sizeof(typename X::T)) % 16 == 0;
+    if (p.planes >= 8)
+        return vec ? launch_rows<X, D, 1, 8, true, true>(p, r, st) : launch_rows<X, D, 1, 8, true, false>(p, r, st);
+    return vec ? launch_rows<X, D, 2, 1, true, true>(p, r, st) : launch_rows<X, D, 2, 1, true, false>(p, r, st);
+}
+template <class X>
+static int linear_rows(const Product &p, const Rows &r, int out_dtype, hipStream_t st) {
+    if (out_dtype == LIRA_DTYPE_F32) return linear_rows<X, F32>(p, r, st);
+    if (out_dtype == LIRA_DTYPE_BF16) return linear_rows<X, BF16>(p, r, st);
+    return linear_rows<X, F16>(p, r, st);
+}
 template <class D>
 static int product(const Product &p, hipStream_t st) {
+    if (p.m <= 16) {
+        const Rows r = {nullptr, 0, 0};
+        if (p.planes >= 8) return launch_rows<F32, D, 1, 8, false, false>(p, r, st);
+        return launch_rows<F32, D, 2, 1, false, false>(p, r, st);
+    }
+    // Rows alone decide while one tile takes them all; then the largest tile that still gives each of
+    // the 256 compute units one (k = n = 8192, us a call with the packing of the rows: 64 rows
+    // 16.4 here, 21 on the 64 x 64 tile; 1024 rows 58 on the 128 x 128 tile, 512 tiles of it).
     const int64_t big = ((p.n + 255) / 256) * ((p.m + 255) / 256), mid = ((p.n + 127) / 128) * ((p.m + 127) / 128);
-    if (big >= 256) return launch_tile<256, 256, 2, 4, D>(p, st);
-    if (mid >= 256) return launch_tile<128, 128, 2, 2, D>(p, st);
-    return launch_tile<64, 64, 2, 2, D>(p, st);
+    if (p.m <= 32) return launch_tile<32, 32, 2, 2, 2, 4, 4, D>(p, st);
+    if (p.m <= 64) return launch_tile<32, 64, 2, 2, 2, 3, 4, D>(p, st);
+    if (big >= 256) return launch_tile<256, 256, 2, 4, 1, 4, 1, D>(p, st);
+    if (mid >= 256) return launch_tile<128, 128, 2, 2, 1, 4, 1, D>(p, st);
+    // (one tile a compute unit: all of its LDS, twice the planes a barrier: 128 rows 18.5 us, else 22)
+    if (((p.n + 63) / 64) * ((p.m + 63) / 64) <= 256) return launch_tile<64, 64, 2, 2, 2, 4, 4, D>(p, st);
+    return launch_tile<64, 64, 2, 2, 2, 4, 2, D>(p, st);
+}
+static int product(const Product &p, int out_dtype, hipStream_t st) {
+    if (out_dtype == LIRA_DTYPE_F32) return product<F32>(p, st);
+    if (out_dtype == LIRA_DTYPE_BF16) return product<BF16>(p, st);
+    return product<F16>(p, st);
 }
 
 static int check_product(int64_t m, int64_t n, int act, const void *out, int out_dtype, int64_t ldo) {
@@ -377,20 +657,11 @@ int lira_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t pla
     if (ld < k) return fail(LIRA_EINVAL, "ld must be at least k");
     if (n == 0) return LIRA_OK;
     if (!out) return fail(LIRA_EINVAL, "NULL buffer");
-    if (int rc = check_grid((n + 15) / 16, "mx4_dequantize")) return rc;
+    if (int rc = check_grid((n + 7) / 8, "mx4_dequantize")) return rc;
     hipStream_t st = (hipStream_t)stream;
-    const dim3 g((unsigned)((n + 15) / 16), (unsigned)planes_of(k));
-    if (dtype == LIRA_DTYPE_F32)
-        hipLaunchKernelGGL((k_mx4_dequantize<F32>), g, dim3(256), 0, st, codes, scales, plane_rows, n, k, (float *)out,
-                           ld);
-    else if (dtype == LIRA_DTYPE_BF16)
-        hipLaunchKernelGGL((k_mx4_dequantize<BF16>), g, dim3(256), 0, st, codes, scales, plane_rows, n, k,
-                           (__bf16 *)out, ld);
-    else
-        hipLaunchKernelGGL((k_mx4_dequantize<F16>), g, dim3(256), 0, st, codes, scales, plane_rows, n, k,
-                           (_Float16 *)out, ld);
-    LIRA_HIP_TRY(hipGetLastError());
-    return LIRA_OK;
+    if (dtype == LIRA_DTYPE_F32) return dequantize<F32>(codes, scales, plane_rows, n, k, out, ld, st);
+    if (dtype == LIRA_DTYPE_BF16) return dequantize<BF16>(codes, scales, plane_rows, n, k, out, ld, st);
+    return dequantize<F16>(codes, scales, plane_rows, n, k, out, ld, st);
 }
 
 int lira_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, int64_t a_plane_rows, int64_t m,
@@ -403,15 +674,13 @@ int lira_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, int64_t a_p
     hipStream_t st = (hipStream_t)stream;
     const Product p = {a_codes, a_scales, b_codes, b_scales, a_plane_rows, b_plane_rows, m, n, ldo,
                        (int)planes_of(k), {bias, alpha, act}, out};
-    if (out_dtype == LIRA_DTYPE_F32) return product<F32>(p, st);
-    if (out_dtype == LIRA_DTYPE_BF16) return product<BF16>(p, st);
-    return product<F16>(p, st);
+    return product(p, out_dtype, st);
 }
 
 int lira_mx4_linear_workspace_size(int64_t m, int64_t n, int64_t k, size_t *bytes) {
     if (!bytes) return fail(LIRA_EINVAL, "NULL buffer");
     if (m < 0 || n < 0 || k <= 0) return fail(LIRA_EINVAL, "bad shape");
-    *bytes = m == 0 || n == 0 ? 0 : (size_t)(planes_of(k) * m * 68);
+    *bytes = m == 0 || n == 0 || fused_rows(m, k) ? 0 : (size_t)(planes_of(k) * m * 68);
     return LIRA_OK;
 }
 
@@ -429,6 +698,14 @@ int lira_mx4_linear(const void *x, int dtype, int64_t m, int64_t k, int64_t ldx,
     if (int rc = lira_mx4_linear_workspace_size(m, n, k, &need)) return rc;
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
         return fail(LIRA_EINVAL, "workspace too small (lira_mx4_linear_workspace_size) or not 16-byte aligned");
+    if (!need) {
+        const Product p = {nullptr, nullptr, b_codes, b_scales, 0, b_plane_rows, m, n, ldo,
+                           (int)planes_of(k), {bias, alpha, act}, out};
+        const Rows r = {x, k, ldx};
+        if (dtype == LIRA_DTYPE_F32) return linear_rows<F32>(p, r, out_dtype, (hipStream_t)stream);
+        if (dtype == LIRA_DTYPE_BF16) return linear_rows<BF16>(p, r, out_dtype, (hipStream_t)stream);
+        return linear_rows<F16>(p, r, out_dtype, (hipStream_t)stream);
+    }
     uint8_t *ac = (uint8_t *)workspace, *as = ac + planes_of(k) * m * 64;
     if (int rc = lira_mx4_quantize(x, dtype, m, k, ldx, ac, as, m, stream)) return rc;
     return lira_mx4_matmul(ac, as, m, m, b_codes, b_scales, b_plane_rows, n, k, alpha, bias, act, out, out_dtype, ldo,

@@ -41,6 +41,15 @@ struct F16 {
 // |v| as an integer: orders like |v| and puts Inf and NaN above every number
 __device__ __forceinline__ uint32_t mag(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// mag() of the largest of a block's 32 elements, 8 in each of 4 neighbouring lanes (DPP)
+__device__ __forceinline__ uint32_t quad_max(const float (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, mag(v[i]));
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0xB1, 0xf, 0xf, false));  // lane ^ 1
+    return max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x4E, 0xf, 0xf, false));  // lane ^ 2
+}
+
 // the scale byte of a block whose largest magnitude has these bits: exponent - 2 (6 = 1.5 * 2^2
 // is the largest element), not below 2^-127; 255 where the block holds Inf or NaN
 __device__ __forceinline__ uint32_t scale_code(uint32_t m) {
@@ -51,7 +60,7 @@ __device__ __forceinline__ uint32_t scale_code(uint32_t m) {
 __device__ __forceinline__ float scale_operand(uint32_t code) { return __uint_as_float(code << 23); }
 
 // 8 floats -> 8 codes, element 0 in the low 4 bits; v / scale to nearest even, saturated at 6
-__device__ __forceinline__ uint32_t to_codes(const float (&v)[8], float scale) {
+__device__ __forceinline__ uint32_t to_codes(const float *v, float scale) {
     uint32_t r = 0;
     r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[0], v[1], scale, 0);
     r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, v[2], v[3], scale, 1);
@@ -60,29 +69,43 @@ __device__ __forceinline__ uint32_t to_codes(const float (&v)[8], float scale) {
     return r;
 }
 
-// the number a code stands for times 2^(s - 127); exact in fp32 (at most 2 mantissa bits)
-__device__ __forceinline__ float from_code(uint32_t c, uint32_t s) {
-    const uint32_t a = c & 7u;
-    float v = a < 2 ? 0.5f * (float)a : __uint_as_float(((a >> 1) + 126u) << 23 | (a & 1u) << 22);
-    v = (c & 8u) ? -v : v;
-    return s == 255 ? __uint_as_float(0x7fc00000u) : ldexpf(v, (int)s - 127);
+// N codes (the first in the low bits) -> the numbers they stand for; exact in fp32 but for 6 * 2^127
+// and its like, which are past fp32's end
+template <int N>
+__device__ __forceinline__ void from_codes(uint32_t c, uint32_t s, float (&v)[N]) {
+    const float scale = scale_operand(s);
+    f32x2 t[4];
+    t[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 0);
+    t[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 1);
+    if (N > 4) {
+        t[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 2);
+        t[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 3);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = s == 255 ? __uint_as_float(0x7fc00000u) : t[i / 2][i % 2];
 }
 
-// 8 consecutive elements of a row from element j (zeros past the row's end); VEC: the row's
-// first element and the row stride are multiples of 16 bytes
-template <class D, bool VEC>
-__device__ __forceinline__ void load8(const typename D::T *row, int64_t j, int64_t k, float (&v)[8]) {
+// N = 8 or 32 consecutive elements of a row from element j (zeros past the row's end); VEC: the row's
+// first element and the row stride are multiples of 16 bytes.  The ends of rows read their last
+// element's place again: a branch round every load would wait for each.
+template <class D, bool VEC, int N>
+__device__ __forceinline__ void load_run(const typename D::T *row, int64_t j, int64_t k, float (&v)[N]) {
     typedef typename D::T T;
-    if (VEC && j + 8 <= k) {
+    if (VEC && j + N <= k) {
+        constexpr int E = 16 / sizeof(T);
         struct alignas(16) V {
-            T e[8];
-        };
-        const V t = *reinterpret_cast<const V *>(row + j);
+            T e[E];
+        } t[N / E];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = D::up(t.e[i]);
+        for (int i = 0; i < N / E; ++i) t[i] = *reinterpret_cast<const V *>(row + j + i * E);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = D::up(t[i / E].e[i % E]);
     } else {
+        T t[N];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = j + i < k ? D::up(row[j + i]) : 0.0f;
+        for (int i = 0; i < N; ++i) t[i] = row[j + i < k ? j + i : k - 1];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = j + i < k ? D::up(t[i]) : 0.0f;
     }
 }
 

@@ -154,6 +154,26 @@ def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
 
 
+_functions: dict = {}
+
+
+def run(name: str, *args) -> None:
+    """call() for the operators that a program calls thousands of times a second: the function is
+    looked up once."""
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(load(), name)
+    rc = f(*args)
+    if rc:
+        check(rc, name)
+
+
+def raw_stream(device_index: int) -> int:
+    """The current stream of a device as an address, without a torch.cuda.Stream object for it (3 us)."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def ptr(t) -> int:
     """Device/host pointer of a torch tensor (or None -> NULL)."""
     if t is None:

@@ -15,6 +15,7 @@ whose leaves no eager autograd graph still uses.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -27,89 +28,114 @@ def check_device(logits) -> None:
         raise ValueError("logits must be a tensor on the GPU")
 
 
+def _rows_of(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
+def _fp32(t):
+    """A constant of the kernels: detached, float32, contiguous (None stays None)."""
+    if t is None:
+        return None
+    if t.requires_grad:
+        t = t.detach()
+    return t.to(torch.float32).contiguous()
+
+
+def _row_values(t, name: str, lead, device):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.device != device or t.shape != lead or not t.is_floating_point():
+        raise ValueError(f"{name} must be a {tuple(lead)} float tensor on {device}")
+    return _fp32(t.reshape(-1))
+
+
 def _entries(logits, top_ids, top_logits, temperature, teacher_lse):
-    """The checked arguments, as (rows, vocab) logits and (rows, top) entries."""
+    """(logits (rows, vocab), the logits' leading dimensions, ids, teacher's logits, its logsumexp), checked and as
+    the kernels read them (the teacher is constant)."""
     check_device(logits)
-    if logits.dim() < 1:
+    shape, dev = logits.shape, logits.device
+    if not shape:
         raise ValueError("logits must have at least one dimension")
-    lead, vocab = logits.shape[:-1], logits.shape[-1]
-    z = check_rows(logits.reshape(-1, vocab) if vocab else logits.reshape(lead.numel(), 0), "logits")
+    lead, vocab = shape[:-1], shape[-1]
     if vocab < 1:
         raise ValueError("logits must have at least one output")
+    z = check_rows(_rows_of(logits), "logits")
     for t, name in ((top_ids, "top_ids"), (top_logits, "top_logits")):
-        if not isinstance(t, torch.Tensor) or t.device != z.device:
-            raise ValueError(f"{name} must be a tensor on {z.device}")
-        if t.dim() != logits.dim() or t.shape[:-1] != lead:
+        if not isinstance(t, torch.Tensor) or t.device != dev:
+            raise ValueError(f"{name} must be a tensor on {dev}")
+        if t.shape[:-1] != lead or t.dim() != logits.dim():
             raise ValueError(f"{name} must have the logits' leading dimensions {tuple(lead)}, not {tuple(t.shape[:-1])}")
-    if top_ids.dtype not in (torch.int32, torch.int64):
+    if top_ids.dtype != torch.int32 and top_ids.dtype != torch.int64:
         raise ValueError(f"top_ids must be int32 or int64, not {top_ids.dtype}")
     if top_logits.dtype not in DTYPES:
         raise ValueError(f"top_logits must be float32, bfloat16 or float16, not {top_logits.dtype}")
-    top = top_ids.shape[-1]
-    if top < 1 or top_logits.shape != top_ids.shape:
+    if top_ids.shape[-1] < 1 or top_logits.shape != top_ids.shape:
         raise ValueError(f"top_ids {tuple(top_ids.shape)} and top_logits {tuple(top_logits.shape)} must have the same "
                          "shape, at least one entry a row")
-    if not 0.0 < float(temperature) < float("inf"):
+    if not 0.0 < temperature < float("inf"):
         raise ValueError("temperature must be positive and finite")
-    if teacher_lse is not None and (not isinstance(teacher_lse, torch.Tensor) or teacher_lse.device != z.device
-                                    or teacher_lse.shape != lead or not teacher_lse.is_floating_point()):
-        raise ValueError(f"teacher_lse must be a {tuple(lead)} float tensor on {z.device}")
-    return z, lead, top
-
-
-def _plain(top_ids, top_logits, teacher_lse, top):
-    """The entries as the kernels read them (constants: the teacher gets no gradient)."""
-    ids = top_ids.reshape(-1, top).contiguous()
-    tv = top_logits.detach().reshape(-1, top).to(torch.float32).contiguous()
-    lse = None if teacher_lse is None else teacher_lse.detach().reshape(-1).to(torch.float32).contiguous()
-    return ids, tv, lse
+    return (z, lead, _rows_of(top_ids).contiguous(), _fp32(_rows_of(top_logits)),
+            _row_values(teacher_lse, "teacher_lse", lead, dev))
 
 
 def _head(z, ld, ids, tv, lse, t):
     rows, vocab = z.shape
     return (z.data_ptr(), DTYPES[z.dtype], rows, vocab, ld, ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32,
-            tv.data_ptr(), ids.shape[1], t, _lib.ptr(lse))
+            tv.data_ptr(), ids.shape[1], t, None if lse is None else lse.data_ptr())
 
 
-def _workspace(z, ids):
+@functools.lru_cache(maxsize=1024)
+def _workspace_size(rows: int, vocab: int, top: int, dtype: int) -> int:
     need = ctypes.c_size_t()
-    _lib.call("lira_distill_workspace_size", *z.shape, ids.shape[1], DTYPES[z.dtype], ctypes.byref(need))
-    return torch.empty(need.value, dtype=torch.uint8, device=z.device) if need.value else None
+    _lib.run("lira_distill_workspace_size", rows, vocab, top, dtype, ctypes.byref(need))
+    return need.value
+
+
+def _forward(z, ids, tv, lse, t, stats, row_weight, dz):
+    z, ld = _rows(z)
+    rows, vocab = z.shape
+    dev = z.device
+    loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    need = _workspace_size(rows, vocab, ids.shape[1], DTYPES[z.dtype])
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    _lib.run("lira_distill_topk", *_head(z, ld, ids, tv, lse, t), loss.data_ptr(), _lib.ptr(stats), _lib.ptr(row_weight),
+             1, _lib.ptr(dz), vocab, _lib.ptr(ws), need, _lib.raw_stream(dev.index))
+    return loss
 
 
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, ids, tv, lse, t, reduction):
-        z, ld = _rows(z)
-        rows = z.shape[0]
-        loss = torch.empty(rows, dtype=torch.float32, device=z.device)
-        stats = torch.empty((rows, 4), dtype=torch.float32, device=z.device)
-        ws = _workspace(z, ids)
-        _lib.call("lira_distill_topk", *_head(z, ld, ids, tv, lse, t), loss.data_ptr(), stats.data_ptr(), None, 0, None,
-                  0, _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_ptr())
+        rows, dev = z.shape[0], z.device
+        stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
+        loss = _forward(z, ids, tv, lse, t, stats, None, None)
         ctx.save_for_backward(z, ids, tv, lse, stats)
         ctx.t, ctx.factor = t, None
         if reduction == "none":
             return loss
-        out = torch.empty(2, dtype=torch.float32, device=z.device)
-        _lib.call("lira_distill_reduce", loss.data_ptr(), stats.data_ptr(), rows, reduction == "mean", out.data_ptr(),
-                  _lib.stream_ptr())
+        out = torch.empty(2, dtype=torch.float32, device=dev)
+        _lib.run("lira_distill_reduce", loss.data_ptr(), stats.data_ptr(), rows, reduction == "mean", out.data_ptr(),
+                 _lib.raw_stream(dev.index))
         ctx.factor = out[1]
         return out[0].clone()
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        if torch.is_grad_enabled():
+            raise RuntimeError("distill_topk_loss has no second derivative (create_graph=True)")
         z, ids, tv, lse, stats = ctx.saved_tensors
         rows, vocab = z.shape
-        with on(z.device):
-            g = (g if ctx.factor is None else g * ctx.factor).to(torch.float32)
+        dev = z.device
+        with on(dev):
+            if ctx.factor is not None:
+                g = g * ctx.factor
             whole = g.dim() == 0 or (rows > 1 and g.stride(0) == 0)  # one factor for all rows
-            g = g if whole else g.contiguous()
+            if not whole:
+                g = g.contiguous()
             z, ld = _rows(z)
-            dz = torch.empty((rows, vocab), dtype=z.dtype, device=z.device)
-            _lib.call("lira_distill_topk_backward", *_head(z, ld, ids, tv, lse, ctx.t), stats.data_ptr(), g.data_ptr(),
-                      0 if whole else 1, dz.data_ptr(), vocab, _lib.stream_ptr())
+            dz = torch.empty((rows, vocab), dtype=z.dtype, device=dev)
+            _lib.run("lira_distill_topk_backward", *_head(z, ld, ids, tv, lse, ctx.t), stats.data_ptr(), g.data_ptr(),
+                     0 if whole else 1, dz.data_ptr(), vocab, _lib.raw_stream(dev.index))
         return dz, None, None, None, None, None
 
 
@@ -127,10 +153,11 @@ def distill_topk_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_logits: t
     """
     if reduction not in ("none", "sum", "mean"):
         raise ValueError(f"reduction must be 'none', 'sum' or 'mean', not {reduction!r}")
-    z, lead, top = _entries(logits, top_ids, top_logits, temperature, teacher_lse)
-    with on(z.device):
-        loss = _Loss.apply(z, *_plain(top_ids, top_logits, teacher_lse, top), float(temperature), reduction)
-    return loss.view(lead) if reduction == "none" else loss
+    check_device(logits)
+    with on(logits.device):
+        z, lead, ids, tv, lse = _entries(logits, top_ids, top_logits, temperature, teacher_lse)
+        loss = _Loss.apply(z, ids, tv, lse, temperature, reduction)
+    return loss.view(lead) if reduction == "none" and len(lead) != 1 else loss
 
 
 @torch.no_grad()
@@ -143,23 +170,16 @@ def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_
     ``logits.backward(grad)``.  row_weight (...): None = 1.  grad_out: where the gradient goes, a
     contiguous tensor like the logits; the logits themselves are allowed."""
     check_device(logits)
-    with on(logits.device, stream):
-        z, lead, top = _entries(logits, top_ids, top_logits, temperature, teacher_lse)
-        if row_weight is not None and (not isinstance(row_weight, torch.Tensor) or row_weight.device != z.device
-                                       or row_weight.shape != lead or not row_weight.is_floating_point()):
-            raise ValueError(f"row_weight must be a {tuple(lead)} float tensor on {z.device}")
-        if grad_out is not None and (not isinstance(grad_out, torch.Tensor) or grad_out.shape != logits.shape
-                                     or grad_out.dtype != logits.dtype or grad_out.device != z.device
-                                     or not grad_out.is_contiguous()):
+    dev = logits.device
+    with on(dev, stream):
+        z, lead, ids, tv, lse = _entries(logits, top_ids, top_logits, temperature, teacher_lse)
+        w = _row_values(row_weight, "row_weight", lead, dev)
+        if grad_out is None:
+            dz = torch.empty(logits.shape, dtype=z.dtype, device=dev)
+        elif not isinstance(grad_out, torch.Tensor) or grad_out.shape != logits.shape or grad_out.dtype != z.dtype \
+                or grad_out.device != dev or not grad_out.is_contiguous():
             raise ValueError("grad_out must be a contiguous tensor of the logits' shape, type and device")
-        z, ld = _rows(z.detach())
-        rows, vocab = z.shape
-        ids, tv, lse = _plain(top_ids, top_logits, teacher_lse, top)
-        w = None if row_weight is None else row_weight.detach().reshape(-1).to(torch.float32).contiguous()
-        loss = torch.empty(rows, dtype=torch.float32, device=z.device)
-        dz = torch.empty((rows, vocab), dtype=z.dtype, device=z.device) if grad_out is None else grad_out
-        ws = _workspace(z, ids)
-        _lib.call("lira_distill_topk", *_head(z, ld, ids, tv, lse, float(temperature)), loss.data_ptr(), None,
-                  _lib.ptr(w), 1, dz.data_ptr(), vocab, _lib.ptr(ws), 0 if ws is None else ws.numel(),
-                  _lib.stream_ptr())
-    return loss.view(lead), dz.view(logits.shape)
+        else:
+            dz = grad_out
+        loss = _forward(z, ids, tv, lse, temperature, None, w, dz)
+    return loss if len(lead) == 1 else loss.view(lead), dz

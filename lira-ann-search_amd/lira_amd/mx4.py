@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -26,6 +27,9 @@ DTYPES = {torch.float32: _lib.LIRA_DTYPE_F32, torch.bfloat16: _lib.LIRA_DTYPE_BF
 ACTIVATIONS = {None: _lib.LIRA_ACT_NONE, "relu": _lib.LIRA_ACT_RELU, "sigmoid": _lib.LIRA_ACT_SIGMOID}
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on(device: torch.device, stream=None):
     """The context a call runs in: the tensors' device, and ``stream`` as the current one, so that
     whatever the call allocates belongs to the stream that uses it."""
@@ -33,9 +37,7 @@ def on(device: torch.device, stream=None):
         if stream.device != device:
             raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
         return torch.cuda.stream(stream)
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def check_rows(x, name: str, device=None) -> torch.Tensor:
@@ -55,14 +57,15 @@ def check_rows(x, name: str, device=None) -> torch.Tensor:
 def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """x with consecutive elements in its rows, and its row stride."""
     n, k = x.shape
-    if x.stride(1) == 1 and (n <= 1 or x.stride(0) >= k):
-        return x, k if n <= 1 else x.stride(0)
+    s0, s1 = x.stride()
+    if s1 == 1 and (s0 >= k or n <= 1):
+        return x, k if n <= 1 else s0
     x = x.contiguous()
     return x, k
 
 
-def _no_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_grad(t) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("the 4-bit operators have no gradient: call them under torch.no_grad() or on detached tensors")
 
 
@@ -87,6 +90,13 @@ class MX4Tensor:
                 scales.clone(memory_format=torch.contiguous_format)
             rows = codes.shape[1]
         self.codes, self.scales, self.k, self.plane_rows = codes, scales, k, rows
+
+    @classmethod
+    def _made(cls, codes, scales, k) -> "MX4Tensor":
+        """Of two contiguous tensors that this module has just made."""
+        t = object.__new__(cls)
+        t.codes, t.scales, t.k, t.plane_rows = codes, scales, k, codes.shape[1]
+        return t
 
     @staticmethod
     def _plane_rows(t: torch.Tensor):
@@ -132,27 +142,26 @@ def mx4_quantize(x: torch.Tensor, stream=None) -> MX4Tensor:
     if k < 1:
         raise ValueError("x must have at least one column")
     p = (k + 127) // 128
-    with on(x.device, stream):
+    dev = x.device
+    with on(dev, stream):
         x, ld = _rows(x)
-        codes = torch.empty((p, n, 64), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((p, n, 4), dtype=torch.uint8, device=x.device)
-        _lib.call("lira_mx4_quantize", x.data_ptr(), DTYPES[x.dtype], n, k, ld, codes.data_ptr(), scales.data_ptr(), n,
-                  _lib.stream_ptr())
-    return MX4Tensor(codes, scales, k)
+        codes = torch.empty((p, n, 64), dtype=torch.uint8, device=dev)
+        scales = torch.empty((p, n, 4), dtype=torch.uint8, device=dev)
+        _lib.run("lira_mx4_quantize", x.data_ptr(), DTYPES[x.dtype], n, k, ld, codes.data_ptr(), scales.data_ptr(), n,
+                 _lib.raw_stream(dev.index))
+    return MX4Tensor._made(codes, scales, k)
 
 
-def _out(out, shape, dtype, device) -> torch.Tensor:
+def _out(out, shape, dtype, device) -> tuple[torch.Tensor, int]:
+    """Where the result goes, and its row stride."""
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty(shape, dtype=dtype, device=device), max(1, shape[1])
     if not isinstance(out, torch.Tensor) or out.device != device or out.dtype != dtype or tuple(out.shape) != shape:
         raise ValueError(f"out must be a {shape} {dtype} tensor on {device}")
     if shape[1] > 1 and out.stride(1) != 1 or shape[0] > 1 and out.stride(0) < shape[1]:
         raise ValueError("out must have rows of consecutive elements that do not overlap")
-    return out
-
-
-def _ld(out: torch.Tensor) -> int:
-    return out.stride(0) if out.shape[0] > 1 else max(1, out.shape[1])
+    _no_grad(out)
+    return out, out.stride(0) if shape[0] > 1 else max(1, shape[1])
 
 
 def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
@@ -162,11 +171,11 @@ def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float32, out: torch.
         raise ValueError("t must be an MX4Tensor")
     if dtype not in DTYPES:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
-    with on(t.device, stream):
-        out = _out(out, t.shape, dtype, t.device)
-        _no_grad(out)
-        _lib.call("lira_mx4_dequantize", t.codes.data_ptr(), t.scales.data_ptr(), t.plane_rows, t.shape[0], t.k,
-                  out.data_ptr(), DTYPES[dtype], _ld(out), _lib.stream_ptr())
+    dev, n = t.codes.device, t.codes.shape[1]
+    with on(dev, stream):
+        out, ld = _out(out, (n, t.k), dtype, dev)
+        _lib.run("lira_mx4_dequantize", t.codes.data_ptr(), t.scales.data_ptr(), t.plane_rows, n, t.k, out.data_ptr(),
+                 DTYPES[dtype], ld, _lib.raw_stream(dev.index))
     return out
 
 
@@ -197,14 +206,21 @@ def mx4_matmul(a: MX4Tensor, b: MX4Tensor, bias: torch.Tensor | None = None, act
     if out_dtype not in DTYPES:
         raise ValueError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
     m, n = a.shape[0], b.shape[0]
-    with on(a.device, stream):
+    dev = a.device
+    with on(dev, stream):
         bias = None if bias is None else bias.to(torch.float32).contiguous()
-        out = _out(out, (m, n), out_dtype, a.device)
-        _no_grad(out)
-        _lib.call("lira_mx4_matmul", a.codes.data_ptr(), a.scales.data_ptr(), a.plane_rows, m, b.codes.data_ptr(),
-                  b.scales.data_ptr(), b.plane_rows, n, a.k, float(alpha), _lib.ptr(bias), act, out.data_ptr(),
-                  DTYPES[out_dtype], _ld(out), _lib.stream_ptr())
+        out, ldo = _out(out, (m, n), out_dtype, dev)
+        _lib.run("lira_mx4_matmul", a.codes.data_ptr(), a.scales.data_ptr(), a.plane_rows, m, b.codes.data_ptr(),
+                 b.scales.data_ptr(), b.plane_rows, n, a.k, alpha, _lib.ptr(bias), act, out.data_ptr(),
+                 DTYPES[out_dtype], ldo, _lib.raw_stream(dev.index))
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace(m: int, n: int, k: int) -> int:
+    need = ctypes.c_size_t()
+    _lib.run("lira_mx4_linear_workspace_size", m, n, k, ctypes.byref(need))
+    return need.value
 
 
 def mx4_linear(x: torch.Tensor, w: MX4Tensor, bias: torch.Tensor | None = None, activation: str | None = None,
@@ -220,16 +236,14 @@ def mx4_linear(x: torch.Tensor, w: MX4Tensor, bias: torch.Tensor | None = None, 
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in DTYPES:
         raise ValueError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
-    m, n = x.shape[0], w.shape[0]
-    need = ctypes.c_size_t()
-    _lib.call("lira_mx4_linear_workspace_size", m, n, w.k, ctypes.byref(need))
-    with on(x.device, stream):
+    m, n, k, dev = x.shape[0], w.codes.shape[1], w.k, x.device
+    need = _linear_workspace(m, n, k)
+    with on(dev, stream):
         x, ld = _rows(x)
         bias = None if bias is None else bias.to(torch.float32).contiguous()
-        out = _out(out, (m, n), out_dtype, x.device)
-        _no_grad(out)
-        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device) if need.value else None
-        _lib.call("lira_mx4_linear", x.data_ptr(), DTYPES[x.dtype], m, w.k, ld, w.codes.data_ptr(),
-                  w.scales.data_ptr(), w.plane_rows, n, float(alpha), _lib.ptr(bias), act, out.data_ptr(),
-                  DTYPES[out_dtype], _ld(out), _lib.ptr(ws), need.value, _lib.stream_ptr())
+        out, ldo = _out(out, (m, n), out_dtype, dev)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _lib.run("lira_mx4_linear", x.data_ptr(), DTYPES[x.dtype], m, k, ld, w.codes.data_ptr(), w.scales.data_ptr(),
+                 w.plane_rows, n, alpha, _lib.ptr(bias), act, out.data_ptr(), DTYPES[out_dtype], ldo, _lib.ptr(ws), need,
+                 _lib.raw_stream(dev.index))
     return out
