@@ -16,13 +16,13 @@ liblira_hip.so), with the reference's Python-side interfaces on top:
 from ._lib import LiraError, load as load_library  # noqa: F401
 from .index import (PartitionedIndex, build_csr, centroid_dist, centroid_gemm,  # noqa: F401
                     normalize_metric, order_probes, rank_nearest, select_probes, RankWorkspace)
-from .faiss_compat import IndexFlatIP, IndexFlatL2  # noqa: F401
+from .faiss_compat import IndexFlatIP, IndexFlatL2, IndexMX4  # noqa: F401
 from .mx4 import MX4Tensor, mx4_dequantize, mx4_linear, mx4_matmul, mx4_quantize  # noqa: F401
 from .distill import distill_topk_loss, distill_topk_loss_and_grad  # noqa: F401
 
 __all__ = [
     "LiraError", "PartitionedIndex", "build_csr", "centroid_dist", "centroid_gemm",
-    "rank_nearest", "select_probes", "order_probes", "normalize_metric", "IndexFlatL2", "IndexFlatIP",
+    "rank_nearest", "select_probes", "order_probes", "normalize_metric", "IndexFlatL2", "IndexFlatIP", "IndexMX4",
     "RankWorkspace", "load_library", "MX4Tensor", "mx4_quantize", "mx4_dequantize", "mx4_matmul", "mx4_linear",
     "distill_topk_loss", "distill_topk_loss_and_grad",
 ]

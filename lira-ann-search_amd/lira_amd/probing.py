@@ -3,9 +3,10 @@
 LIRA scores every partition with a two-tower MLP (model_probing.py:5-39):
 sigmoid(fc([dist_tower(standardised centroid distances) || vec_tower(query)])).
 It is *called* on the query path (search.cpp:430-445) but it is a handful of
-small dense layers, so it runs as a PyTorch-ROCm module (hipBLASLt GEMMs), not
-a hand-written kernel.  Parameter names match MLP_2_Input, so a state_dict or a
-TorchScript file trained by the reference loads unchanged.
+small dense layers, so it runs as a PyTorch-ROCm module (hipBLASLt GEMMs) by
+default; ``MX4Probe`` is its 4-bit form on the library's own kernels.  Parameter
+names match MLP_2_Input, so a state_dict or a TorchScript file trained by the
+reference loads unchanged.
 """
 from __future__ import annotations
 
@@ -28,6 +29,42 @@ class MLP_2_Input(nn.Module):  # noqa: N801 - reference class name, kept for dro
 
     def forward(self, x_dist: torch.Tensor, x_vec: torch.Tensor) -> torch.Tensor:
         return self.fc(torch.cat((self.distance_net(x_dist), self.vector_net(x_vec)), dim=1))
+
+    def logits(self, x_dist: torch.Tensor, x_vec: torch.Tensor) -> torch.Tensor:
+        """The scores before the sigmoid: what a distillation loss takes."""
+        return self.fc[:-1](torch.cat((self.distance_net(x_dist), self.vector_net(x_vec)), dim=1))
+
+
+class MX4Probe(nn.Module):
+    """A trained probing model in 4 bits: the layers of MLP_2_Input (model_probing.py:5-39) with
+    packed weights, the activations packed on the way into each (lira_mx4_linear: bias and ReLU or
+    sigmoid in the product's epilogue).  Takes the place of the fp32 model in ``ProbePipeline`` and
+    ``SearchEngine``; inference alone.  ``model``: an MLP_2_Input, or any module with its state_dict
+    (a TorchScript file of the reference), on the GPU.
+    """
+
+    _LAYERS = ("distance_net.0", "distance_net.2", "vector_net.0", "vector_net.2", "fc.0", "fc.2")
+
+    def __init__(self, model: nn.Module):
+        super().__init__()
+        from .mx4 import mx4_quantize
+        state = model.state_dict()
+        missing = [k + e for k in self._LAYERS for e in (".weight", ".bias") if k + e not in state]
+        if missing:
+            raise ValueError(f"MX4Probe needs an MLP_2_Input: the model has no {missing[0]}")
+        with torch.no_grad():
+            self.layers = [(mx4_quantize(state[k + ".weight"].float()), state[k + ".bias"].float().clone())
+                           for k in self._LAYERS]
+
+    @torch.no_grad()
+    def forward(self, x_dist: torch.Tensor, x_vec: torch.Tensor) -> torch.Tensor:
+        from .mx4 import mx4_linear
+        (d0, d2, v0, v2, f0, f2), n = self.layers, x_dist.shape[0]
+        nd = d2[0].shape[0]
+        both = torch.empty((n, nd + v2[0].shape[0]), dtype=torch.float32, device=x_dist.device)
+        mx4_linear(mx4_linear(x_dist.float(), *d0, "relu"), *d2, "relu", out=both[:, :nd])
+        mx4_linear(mx4_linear(x_vec.float(), *v0, "relu"), *v2, "relu", out=both[:, nd:])
+        return mx4_linear(mx4_linear(both, *f0, "relu"), *f2, "sigmoid")
 
 
 class NearestCentroidProbe(nn.Module):
@@ -66,7 +103,8 @@ def standard_scaler(dist: torch.Tensor):
 
 
 def fit_probe_to_nearest(model: nn.Module, dist_scaled_fn, nprobe: int, steps: int = 300, batch: int = 4096,
-                         lr: float = 2e-3, seed: int = 0) -> nn.Module:
+                         lr: float = 2e-3, seed: int = 0, distill_weight: float = 0.0,
+                         temperature: float = 1.0) -> nn.Module:
     """Train MLP_2_Input to score each query's nprobe nearest centroids 1 and
     the rest 0 (BCE, Adam), from batches dist_scaled_fn(batch, step) ->
     (standardised distances (n, B), queries (n, d)).
@@ -76,6 +114,10 @@ def fit_probe_to_nearest(model: nn.Module, dist_scaled_fn, nprobe: int, steps: i
     the query-time hot path), so that the MLP-probed pipeline selects a
     realistic number of partitions at threshold 0.5 instead of a random-init
     model's arbitrary ones.
+
+    distill_weight > 0 adds that much of distill_topk_loss: the exact ranking is
+    the teacher, the nprobe smallest distances (negated) its top logits, so the model
+    also learns the ORDER of the near partitions, which the 0 / 1 targets leave out.
     """
     torch.manual_seed(seed)
     opt = torch.optim.Adam(model.parameters(), lr=lr)
@@ -83,10 +125,16 @@ def fit_probe_to_nearest(model: nn.Module, dist_scaled_fn, nprobe: int, steps: i
     model.train()
     for it in range(steps):
         xd, xq = dist_scaled_fn(batch, it)
-        kth = torch.topk(xd, nprobe, dim=1, largest=False).values[:, -1:]
-        target = (xd <= kth).float()
+        near = torch.topk(xd, nprobe, dim=1, largest=False)
+        target = (xd <= near.values[:, -1:]).float()
         opt.zero_grad(set_to_none=True)
-        loss = lossf(model(xd, xq), target)
+        if distill_weight > 0:
+            from .distill import distill_topk_loss
+            logits = model.logits(xd, xq)
+            loss = lossf(torch.sigmoid(logits), target) + \
+                distill_weight * distill_topk_loss(logits, near.indices, -near.values, temperature)
+        else:
+            loss = lossf(model(xd, xq), target)
         loss.backward()
         opt.step()
     model.eval()

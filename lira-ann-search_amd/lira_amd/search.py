@@ -26,7 +26,7 @@ import torch
 
 from .index import PartitionedIndex, build_csr, centroid_dist, normalize_metric, select_probes
 from .io import load_artifacts, read_fvecs, read_ivecs
-from .probing import probe_scores
+from .probing import MX4Probe, probe_scores
 
 
 def recall_at_k(I: np.ndarray, gt: np.ndarray, k: int) -> np.ndarray:
@@ -58,9 +58,12 @@ def thresholds(t_min: float, t_max: float, t_step: float, cpp_exact: bool = True
 
 
 class SearchEngine:
-    """search.cpp's loaded state: inverted lists, centroids, scaler, model."""
+    """search.cpp's loaded state: inverted lists, centroids, scaler, model.
 
-    def __init__(self, artifacts, metric: str = "L2", device: int = 0, dedup: bool = False):
+    probe: "fp32" runs the probing model as it is; "mx4" its layers in 4 bits
+    (``probing.MX4Probe``: the scores, and so the probed sets, are the 4-bit model's)."""
+
+    def __init__(self, artifacts, metric: str = "L2", device: int = 0, dedup: bool = False, probe: str = "fp32"):
         if isinstance(artifacts, str):
             artifacts = load_artifacts(artifacts, device=f"cuda:{device}")
         self.device = torch.device("cuda", device)
@@ -71,6 +74,10 @@ class SearchEngine:
         self.mean = torch.from_numpy(artifacts["scaler_mean"]).to(dev)
         self.scale = torch.from_numpy(artifacts["scaler_scale"]).to(dev)
         self.model = artifacts["model"].to(dev).eval()
+        if probe not in ("fp32", "mx4"):
+            raise ValueError(f"probe must be 'fp32' or 'mx4', not {probe!r}")
+        if probe == "mx4":
+            self.model = MX4Probe(self.model)
         x = torch.from_numpy(np.ascontiguousarray(artifacts["x_d"])).to(dev)
         d2b = torch.from_numpy(np.ascontiguousarray(artifacts["data_2_bkt"])).to(dev)
         offsets, ids, rep = build_csr(d2b, self.n_bkt)
@@ -254,11 +261,12 @@ def main(argv=None) -> int:
     ap.add_argument("--t_max", type=float, default=0.80)
     ap.add_argument("--t_step", type=float, default=0.02)
     ap.add_argument("--device", type=int, default=0)
+    ap.add_argument("--probe", choices=("fp32", "mx4"), default="fp32", help="the probing model's layers (mx4: 4 bits)")
     ap.add_argument("--dedup", action="store_true", help="keep each gid once (search.cpp does not)")
     a = ap.parse_args(argv)
     try:
         prefix = os.path.join(a.artifacts_dir, a.prefix)
-        eng = SearchEngine(prefix, a.metric, a.device, a.dedup)
+        eng = SearchEngine(prefix, a.metric, a.device, a.dedup, a.probe)
         ddir = os.path.join(a.data_path, a.dataset)
         q = np.ascontiguousarray(read_fvecs(os.path.join(ddir, f"{a.dataset}_query.fvecs")))
         gt = np.ascontiguousarray(read_ivecs(os.path.join(ddir, f"{a.dataset}_groundtruth.ivecs")))
