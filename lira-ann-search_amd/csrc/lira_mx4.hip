@@ -7,6 +7,9 @@
 #include "lira_mx4.hpp"
 
 namespace lira {
+#ifndef BIGT
+#define BIGT 256, 256, 2, 4, 1, 4, 1
+#endif
 
 static constexpr int kPlane = 128;  // elements per plane
 
@@ -200,8 +203,12 @@ struct Tile {
     // fills its job's lanes by repeating its last row)
     static constexpr int kScaleAt = (TN + TM) * 64, kPlaneBytes = kScaleAt + kScaleJobs * 256;
     static constexpr int kBytes = SLOTS * PS * kPlaneBytes;
+    // LDS that the sets' sums, or the rows on their way out (16 a wave, 16 bytes apart), take in the slots' place
+    template <class D>
+    static constexpr int epilogue_bytes() {
+        return WK > 1 ? NW * FN * FM * 1024 : NW * 16 * (TN / WN * (int)sizeof(typename D::T) + 16);
+    }
     static_assert(PS % WK == 0, "the sets split a slot's planes evenly");
-    static_assert(WK == 1 || NW * FN * FM * 1024 <= kBytes, "the sets' sums fit the slots");
 
     struct Frags {
         i32x4 b[FN], a[FM];
@@ -359,7 +366,7 @@ __global__ __launch_bounds__(WN *WM *WK * 64) void k_mx4_tile(Product P, int til
     // 16 rows at a time through LDS, a region a wave, so that a wave writes whole runs of a row: straight from
     // the fragments a bf16 store is runs of 32 bytes, 16 rows apart (8192^3 with them 0.35 ms, so 0.29)
     constexpr int E = 16 / sizeof(T), kRow = TNw + E, kUnits = 16 * TNw / E;
-    static_assert(C::NW * 16 * kRow * (int)sizeof(T) <= C::kBytes, "the waves' regions fit the slots");
+    static_assert(WK > 1 || C::NW * 16 * kRow * (int)sizeof(T) == C::template epilogue_bytes<D>(), "a region a wave");
     __syncthreads();  // (every slot has been read)
     T *stage = reinterpret_cast<T *>(smem) + w * (16 * kRow);
 #pragma unroll
@@ -553,13 +560,17 @@ static int dequantize(const uint8_t *codes, const uint8_t *scales, int64_t plane
 template <int TN, int TM, int WN, int WM, int WK, int SLOTS, int PS, class D>
 static int launch_tile(const Product &p, hipStream_t st) {
     typedef Tile<TN, TM, WN, WM, WK, SLOTS, PS> C;
-    static_assert(C::kBytes <= 163840, "160 KB of LDS");
+    static_assert(C::kBytes <= 163840 && C::template epilogue_bytes<D>() <= C::kBytes, "160 KB of LDS");
     static std::atomic<uint64_t> latch{0};
     const void *fn = (const void *)&k_mx4_tile<TN, TM, WN, WM, WK, SLOTS, PS, D>;
     LIRA_HIP_TRY(set_smem_attr_once(latch, fn, C::kBytes));
+    // (few planes: only the slots that they fill, so that more workgroups share a compute unit:
+    // 10000 x 1024 x 128 20 us -> 14)
+    const int steps = (p.planes + PS - 1) / PS, slots = std::min(SLOTS, steps) * PS * C::kPlaneBytes;
+    const int bytes = std::min<int>(C::kBytes, std::max<int>(slots, C::template epilogue_bytes<D>()));
     const int64_t tn = (p.n + TN - 1) / TN, tm = (p.m + TM - 1) / TM;
     if (tn * tm > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "product: too many tiles for one launch");
-    hipLaunchKernelGGL((k_mx4_tile<TN, TM, WN, WM, WK, SLOTS, PS, D>), dim3((unsigned)(tn * tm)), dim3(C::NW * 64), C::kBytes, st, p,
+    hipLaunchKernelGGL((k_mx4_tile<TN, TM, WN, WM, WK, SLOTS, PS, D>), dim3((unsigned)(tn * tm)), dim3(C::NW * 64), bytes, st, p,
                        (int)tn, (int)tm);
     LIRA_HIP_TRY(hipGetLastError());
     return LIRA_OK;
@@ -609,7 +620,7 @@ static int product(const Product &p, hipStream_t st) {
     const int64_t big = ((p.n + 255) / 256) * ((p.m + 255) / 256), mid = ((p.n + 127) / 128) * ((p.m + 127) / 128);
     if (p.m <= 32) return launch_tile<32, 32, 2, 2, 2, 4, 4, D>(p, st);
     if (p.m <= 64) return launch_tile<32, 64, 2, 2, 2, 3, 4, D>(p, st);
-    if (big >= 256) return launch_tile<256, 256, 2, 4, 1, 4, 1, D>(p, st);
+    if (big >= 256) return launch_tile<BIGT, D>(p, st);
     if (mid >= 256) return launch_tile<128, 128, 2, 2, 1, 4, 1, D>(p, st);
     // (one tile a compute unit: all of its LDS, twice the planes a barrier: 128 rows 18.5 us, else 22)
     if (((p.n + 63) / 64) * ((p.m + 63) / 64) <= 256) return launch_tile<64, 64, 2, 2, 2, 4, 4, D>(p, st);
