@@ -345,8 +345,8 @@ int lira_order_probes(int32_t *probe, int64_t n, int64_t max_probe, const float 
  *   nearest (ties to the even code), saturated at 6.  A block of zeros has scale
  *   byte 0; one that holds Inf or NaN has 255 and codes 0.
  * lira_mx4_dequantize is the inverse (exact in fp32, one rounding to the 16-bit types).
- * All entries: device pointers, stream-ordered, asynchronous, capturable, no
- * state between calls; every output element is written by one call in a fixed
+ * All entries: device pointers of the current device, stream-ordered, asynchronous,
+ * capturable, no state between calls; every output element is written by one call in a fixed
  * order of operations, so results do not vary from run to run.
  */
 int lira_mx4_quantize(const void *x, int dtype, int64_t n, int64_t k, int64_t ld, uint8_t *codes,
@@ -357,7 +357,7 @@ int lira_mx4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t pla
  * out[i, j] = act(alpha * sum_l a[i, l] b[j, l] + bias[j]) of two packed arrays,
  * a (m, k) and b (n, k): fp32 sums on the matrix cores, rounded once to out_dtype.
  * bias: fp32 (n) or NULL.  out (m, n), row stride ldo elements; elements outside
- * it are left as they are.  m <= 1048560.  The 4-bit form of the products that
+ * it are left as they are, and it must not overlap an input.  The 4-bit form of the products that
  * lira_centroid_gemm computes in fp32 (search.cpp:220-235) and of the probing
  * model's layers (model_probing.py:33-39).
  */
@@ -408,7 +408,8 @@ int lira_mx4_linear(const void *x, int dtype, int64_t m, int64_t k, int64_t ldx,
  *   dz        NULL: the loss alone.  scale_stride 0: row_scale holds one factor
  *             for all rows; row_scale NULL: 1
  * fp32 sums in a fixed order (results do not vary from run to run), dz rounded
- * once.  Device pointers, stream-ordered, asynchronous, capturable.
+ * once.  Device pointers of the current device, stream-ordered, asynchronous,
+ * capturable.
  * lira_distill_reduce: out[0] = sum of loss, or (mean) the mean over the rows
  * that count; out[1] = the factor of every row's gradient, 1 or 1 / count.
  */

@@ -7,9 +7,6 @@
 #include "lira_mx4.hpp"
 
 namespace lira {
-#ifndef BIGT
-#define BIGT 256, 256, 2, 4, 1, 4, 1
-#endif
 
 static constexpr int kPlane = 128;  // elements per plane
 
@@ -620,7 +617,7 @@ static int product(const Product &p, hipStream_t st) {
     const int64_t big = ((p.n + 255) / 256) * ((p.m + 255) / 256), mid = ((p.n + 127) / 128) * ((p.m + 127) / 128);
     if (p.m <= 32) return launch_tile<32, 32, 2, 2, 2, 4, 4, D>(p, st);
     if (p.m <= 64) return launch_tile<32, 64, 2, 2, 2, 3, 4, D>(p, st);
-    if (big >= 256) return launch_tile<BIGT, D>(p, st);
+    if (big >= 256) return launch_tile<256, 256, 2, 4, 1, 4, 1, D>(p, st);
     if (mid >= 256) return launch_tile<128, 128, 2, 2, 1, 4, 1, D>(p, st);
     // (one tile a compute unit: all of its LDS, twice the planes a barrier: 128 rows 18.5 us, else 22)
     if (((p.n + 63) / 64) * ((p.m + 63) / 64) <= 256) return launch_tile<64, 64, 2, 2, 2, 4, 4, D>(p, st);
@@ -637,8 +634,8 @@ static int check_product(int64_t m, int64_t n, int act, const void *out, int out
     if (act < LIRA_ACT_NONE || act > LIRA_ACT_SIGMOID) return fail(LIRA_EINVAL, "unknown activation");
     if (ldo < n) return fail(LIRA_EINVAL, "ldo must be at least n");
     if (m > 0 && n > 0 && !out) return fail(LIRA_EINVAL, "NULL buffer");
-    if ((m + 15) / 16 > 65535) return fail(LIRA_EUNSUPPORTED, "m must be at most 1048560");
-    return check_grid((n + 63) / 64, "product");
+    if (m > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "product: too many rows for one launch");
+    return check_grid((n + 15) / 16, "product");
 }
 
 }  // namespace lira

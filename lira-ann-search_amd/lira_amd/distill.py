@@ -78,10 +78,11 @@ def _entries(logits, top_ids, top_logits, temperature, teacher_lse):
             _row_values(teacher_lse, "teacher_lse", lead, dev))
 
 
-def _head(z, ld, ids, tv, lse, t):
+def _head(z, ids, tv, lse, t):
+    """The arguments that the forward and the backward entry begin with (z: rows of consecutive elements)."""
     rows, vocab = z.shape
-    return (z.data_ptr(), DTYPES[z.dtype], rows, vocab, ld, ids.data_ptr(), 64 if ids.dtype == torch.int64 else 32,
-            tv.data_ptr(), ids.shape[1], t, None if lse is None else lse.data_ptr())
+    return (z.data_ptr(), DTYPES[z.dtype], rows, vocab, z.stride(0) if rows > 1 else vocab, ids.data_ptr(),
+            64 if ids.dtype == torch.int64 else 32, tv.data_ptr(), ids.shape[1], t, None if lse is None else lse.data_ptr())
 
 
 @functools.lru_cache(maxsize=1024)
@@ -91,30 +92,30 @@ def _workspace_size(rows: int, vocab: int, top: int, dtype: int) -> int:
     return need.value
 
 
-def _forward(z, ids, tv, lse, t, stats, row_weight, dz):
-    z, ld = _rows(z)
-    rows, vocab = z.shape
-    dev = z.device
+def _forward(head, dev, stats, row_weight, dz):
+    rows, vocab = head[2], head[3]
     loss = torch.empty(rows, dtype=torch.float32, device=dev)
-    need = _workspace_size(rows, vocab, ids.shape[1], DTYPES[z.dtype])
+    need = _workspace_size(rows, vocab, head[8], head[1])
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _lib.run("lira_distill_topk", *_head(z, ld, ids, tv, lse, t), loss.data_ptr(), _lib.ptr(stats), _lib.ptr(row_weight),
-             1, _lib.ptr(dz), vocab, _lib.ptr(ws), need, _lib.raw_stream(dev.index))
+    _lib.run("lira_distill_topk", *head, loss.data_ptr(), _lib.ptr(stats), _lib.ptr(row_weight), 1, _lib.ptr(dz), vocab,
+             _lib.ptr(ws), need, _lib.raw_stream(dev.index))
     return loss
 
 
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, ids, tv, lse, t, reduction):
-        rows, dev = z.shape[0], z.device
-        stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
-        loss = _forward(z, ids, tv, lse, t, stats, None, None)
-        ctx.save_for_backward(z, ids, tv, lse, stats)
-        ctx.t, ctx.factor = t, None
+        dev = z.device
+        z = _rows(z)[0]
+        ctx.head = head = _head(z, ids, tv, lse, t)
+        stats = torch.empty((head[2], 4), dtype=torch.float32, device=dev)
+        loss = _forward(head, dev, stats, None, None)
+        ctx.save_for_backward(z, ids, tv, lse, stats)  # (what the head points to, kept and checked for changes)
+        ctx.factor = None
         if reduction == "none":
             return loss
         out = torch.empty(2, dtype=torch.float32, device=dev)
-        _lib.run("lira_distill_reduce", loss.data_ptr(), stats.data_ptr(), rows, reduction == "mean", out.data_ptr(),
+        _lib.run("lira_distill_reduce", loss.data_ptr(), stats.data_ptr(), head[2], reduction == "mean", out.data_ptr(),
                  _lib.raw_stream(dev.index))
         ctx.factor = out[1]
         return out[0].clone()
@@ -123,19 +124,18 @@ class _Loss(torch.autograd.Function):
     def backward(ctx, g):
         if torch.is_grad_enabled():
             raise RuntimeError("distill_topk_loss has no second derivative (create_graph=True)")
-        z, ids, tv, lse, stats = ctx.saved_tensors
-        rows, vocab = z.shape
-        dev = z.device
+        z, _, _, _, stats = ctx.saved_tensors
+        head, dev = ctx.head, z.device
+        rows, vocab = head[2], head[3]
         with on(dev):
             if ctx.factor is not None:
                 g = g * ctx.factor
             whole = g.dim() == 0 or (rows > 1 and g.stride(0) == 0)  # one factor for all rows
             if not whole:
                 g = g.contiguous()
-            z, ld = _rows(z)
             dz = torch.empty((rows, vocab), dtype=z.dtype, device=dev)
-            _lib.run("lira_distill_topk_backward", *_head(z, ld, ids, tv, lse, ctx.t), stats.data_ptr(), g.data_ptr(),
-                     0 if whole else 1, dz.data_ptr(), vocab, _lib.raw_stream(dev.index))
+            _lib.run("lira_distill_topk_backward", *head, stats.data_ptr(), g.data_ptr(), 0 if whole else 1,
+                     dz.data_ptr(), vocab, _lib.raw_stream(dev.index))
         return dz, None, None, None, None, None
 
 
@@ -181,5 +181,6 @@ def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_
             raise ValueError("grad_out must be a contiguous tensor of the logits' shape, type and device")
         else:
             dz = grad_out
-        loss = _forward(z, ids, tv, lse, temperature, None, w, dz)
+        z = _rows(z)[0]  # (perhaps a copy: held until the launch, the head has its address alone)
+        loss = _forward(_head(z, ids, tv, lse, temperature), dev, None, w, dz)
     return loss if len(lead) == 1 else loss.view(lead), dz

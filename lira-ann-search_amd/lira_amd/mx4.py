@@ -152,14 +152,25 @@ def mx4_quantize(x: torch.Tensor, stream=None) -> MX4Tensor:
     return MX4Tensor._made(codes, scales, k)
 
 
-def _out(out, shape, dtype, device) -> tuple[torch.Tensor, int]:
-    """Where the result goes, and its row stride."""
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses from t's first element to past its last one."""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _out(out, shape, dtype, device, *inputs) -> tuple[torch.Tensor, int]:
+    """Where the result goes, and its row stride; not over an input, which other workgroups still read."""
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device), max(1, shape[1])
     if not isinstance(out, torch.Tensor) or out.device != device or out.dtype != dtype or tuple(out.shape) != shape:
         raise ValueError(f"out must be a {shape} {dtype} tensor on {device}")
     if shape[1] > 1 and out.stride(1) != 1 or shape[0] > 1 and out.stride(0) < shape[1]:
         raise ValueError("out must have rows of consecutive elements that do not overlap")
+    lo, hi = _span(out)
+    for t in inputs:
+        if t is not None and lo < _span(t)[1] and _span(t)[0] < hi:
+            raise ValueError("out must not share memory with an input")
     _no_grad(out)
     return out, out.stride(0) if shape[0] > 1 else max(1, shape[1])
 
@@ -173,7 +184,7 @@ def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float32, out: torch.
         raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
     dev, n = t.codes.device, t.codes.shape[1]
     with on(dev, stream):
-        out, ld = _out(out, (n, t.k), dtype, dev)
+        out, ld = _out(out, (n, t.k), dtype, dev, t.codes, t.scales)
         _lib.run("lira_mx4_dequantize", t.codes.data_ptr(), t.scales.data_ptr(), t.plane_rows, n, t.k, out.data_ptr(),
                  DTYPES[dtype], ld, _lib.raw_stream(dev.index))
     return out
@@ -209,7 +220,7 @@ def mx4_matmul(a: MX4Tensor, b: MX4Tensor, bias: torch.Tensor | None = None, act
     dev = a.device
     with on(dev, stream):
         bias = None if bias is None else bias.to(torch.float32).contiguous()
-        out, ldo = _out(out, (m, n), out_dtype, dev)
+        out, ldo = _out(out, (m, n), out_dtype, dev, a.codes, a.scales, b.codes, b.scales, bias)
         _lib.run("lira_mx4_matmul", a.codes.data_ptr(), a.scales.data_ptr(), a.plane_rows, m, b.codes.data_ptr(),
                  b.scales.data_ptr(), b.plane_rows, n, a.k, alpha, _lib.ptr(bias), act, out.data_ptr(),
                  DTYPES[out_dtype], ldo, _lib.raw_stream(dev.index))
@@ -241,7 +252,7 @@ def mx4_linear(x: torch.Tensor, w: MX4Tensor, bias: torch.Tensor | None = None, 
     with on(dev, stream):
         x, ld = _rows(x)
         bias = None if bias is None else bias.to(torch.float32).contiguous()
-        out, ldo = _out(out, (m, n), out_dtype, dev)
+        out, ldo = _out(out, (m, n), out_dtype, dev, x, w.codes, w.scales, bias)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.run("lira_mx4_linear", x.data_ptr(), DTYPES[x.dtype], m, k, ld, w.codes.data_ptr(), w.scales.data_ptr(),
                  w.plane_rows, n, alpha, _lib.ptr(bias), act, out.data_ptr(), DTYPES[out_dtype], ldo, _lib.ptr(ws), need,

@@ -103,6 +103,19 @@ def test_reductions(reduction):
     assert not z.grad[::3].any()
 
 
+def test_no_second_derivative():
+    from lira_amd import distill_topk_loss
+    z, ti, tv, _ = make(5, 70, 4)
+    z.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(distill_topk_loss(z, ti, tv), z, create_graph=True)
+    loss = distill_topk_loss(z, ti, tv)
+    with torch.no_grad():
+        z.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_no_row_counts():
     from lira_amd import distill_topk_loss
     z, ti, tv, _ = make(5, 70, 4)
@@ -145,6 +158,21 @@ def test_special_rows(vocab):
     p = torch.softmax(tv[0].double() / 2, 0)
     check_grad(dz[0], torch.zeros(vocab, device="cuda", dtype=torch.float64).scatter_add_(0, ti[0], -2 * p),
                torch.full((vocab,), 1e-5, device="cuda"))
+
+
+def test_more_entries_than_outputs():
+    """Every output named several times, in rows of every layout (a wave's, a workgroup's, slices)."""
+    from lira_amd import distill_topk_loss_and_grad
+    g = torch.Generator(device="cuda").manual_seed(8)
+    for rows, vocab, top in ((5, 3, 60), (600, 2, 64), (7, 33, 500), (2, 20000, 700)):
+        z = torch.randn(rows, vocab, generator=g, device="cuda")
+        ti = torch.randint(0, min(vocab, 9), (rows, top), generator=g, device="cuda")
+        tv = torch.randn(rows, top, generator=g, device="cuda")
+        loss, grad, tl, tg = ref(z, ti, tv, 1.0)
+        got, dz = distill_topk_loss_and_grad(z, ti, tv)
+        # (an output named up to `top` times: that many additions more)
+        check_loss(got, loss, tl + loss.abs() * top * 2.0 ** -24)
+        check_grad(dz, grad, tg + top * 2.0 ** -24)
 
 
 def test_teacher_lse():

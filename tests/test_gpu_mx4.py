@@ -261,6 +261,17 @@ def test_linear_on_a_stream_and_in_a_graph():
         assert torch.equal(v, mx4_quantize(xs[i]).dequantize())
 
 
+def test_many_rows():
+    """More rows than a grid's second dimension would hold tiles of 16."""
+    from lira_amd import mx4_linear, mx4_quantize
+    g = gen(6)
+    x = torch.randn(1 << 21, 40, generator=g, device="cuda").bfloat16()
+    w = mx4_quantize(torch.randn(20, 40, generator=g, device="cuda"))
+    y = mx4_linear(x, w)
+    at = torch.tensor([0, 1, 77777, (1 << 20) + 5, (1 << 21) - 2, (1 << 21) - 1], device="cuda")
+    check_product(y[at], ref_pack(x[at])[0], w.dequantize().double().cpu().numpy(), 1.0, None, None, torch.bfloat16)
+
+
 def test_more_than_2_31_elements():
     from lira_amd import mx4_linear, mx4_quantize
     g = gen(5)
@@ -302,6 +313,11 @@ def test_refusals():
                        (lambda: w.dequantize(torch.float64), "dtype")):
         with pytest.raises(ValueError, match=text):
             call()
+    buf = torch.randn(4, 409, device="cuda")
+    with pytest.raises(ValueError, match="share memory"):
+        mx4_linear(buf[:, :200], w, out=buf[:, 200:209])  # (between the rows: the spans overlap)
+    with pytest.raises(ValueError, match="share memory"):
+        mx4_linear(x, w, out=x.view(-1)[:36].view(4, 9))
     with pytest.raises(TypeError):
         w[::2]
     with torch.no_grad():
