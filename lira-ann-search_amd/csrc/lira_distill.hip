@@ -430,41 +430,47 @@ static int launch(const DistillArgs &a, hipStream_t st) {
     return LIRA_OK;
 }
 
-// slices of a row: enough workgroups for the 256 compute units where there are few long rows
+// Slices of a row, where there are few long ones: 192 rows keep the 256 compute units busy by themselves
+// (131072 outputs in bf16, us: 128 rows 28 in slices, 33 in whole rows; 256 rows 51 and 33).
+static constexpr int kFewRows = 192;
 static int64_t distill_slices(int64_t rows, int64_t vecs) {
-    if (rows <= 0) return 1;
-    return std::max<int64_t>(1, std::min((vecs + kSliceVecs - 1) / kSliceVecs, rows >= 512 ? 1 : (vecs + kSliceVecs - 1) / kSliceVecs));
+    return rows < 1 || rows >= kFewRows ? 1 : std::max<int64_t>(1, (vecs + kSliceVecs - 1) / kSliceVecs);
 }
 
 template <class D>
 static int run(DistillArgs a, bool grad_only, hipStream_t st) {
     const int64_t vecs = a.vocab / Vec<D>::E;
     const bool few = a.top <= 64;
+    // A row to a wave where rows alone fill the chip or a wave reads it in two loads, else to a workgroup, which gets
+    // it done sooner (loss and gradient, us by waves and by workgroups: 64 x 4096 bf16 8.4 and 5.7, 1024 x 8192
+    // bf16 16.5 and 13.3, 16384 x 1024 fp32 31.7 and 41.8).
+    const bool waves = vecs <= 64 * 2 || a.rows >= 4096;
     if (grad_only) {
-        if (vecs <= 64 * 16 && few) return launch<D, 64, 0, 64, kGrad>(a, st);
+        if (waves && vecs <= 64 * 16 && few) return launch<D, 64, 0, 64, kGrad>(a, st);
         a.slices = (int)std::max<int64_t>(1, (vecs + kSliceVecs - 1) / kSliceVecs);
         return few ? launch<D, 256, 0, 64, kGrad>(a, st) : launch<D, 256, 0, kMaxTop, kGrad>(a, st);
     }
     if (a.slices > 1) {
         if (int rc = launch<D, 256, 0, 64, kPart>(a, st)) return rc;
-        if (!a.dz) {
-            // (the loss alone: one group a row)
-            return few ? launch<D, 256, 0, 64, kJoin>(a, st) : launch<D, 256, 0, kMaxTop, kJoin>(a, st);
-        }
         return few ? launch<D, 256, 0, 64, kJoin>(a, st) : launch<D, 256, 0, kMaxTop, kJoin>(a, st);
     }
     if (!a.dz) {
-        if (vecs <= 64 * 16 && few) return launch<D, 64, 0, 64, kLoss>(a, st);
+        if (waves && vecs <= 64 * 16 && few) return launch<D, 64, 0, 64, kLoss>(a, st);
         return few ? launch<D, 256, 0, 64, kLoss>(a, st) : launch<D, 256, 0, kMaxTop, kLoss>(a, st);
     }
     if (!few) return launch<D, 256, 0, kMaxTop, kBoth>(a, st);
-    // the row in registers: a wave's up to 16 vectors a lane, then 256 and 1024 threads'
+    // (the row in registers)
     if (vecs < 1) return launch<D, 64, 0, 64, kBoth>(a, st);
     if (vecs <= 64) return launch<D, 64, 1, 64, kBoth>(a, st);
     if (vecs <= 64 * 2) return launch<D, 64, 2, 64, kBoth>(a, st);
-    if (vecs <= 64 * 4) return launch<D, 64, 4, 64, kBoth>(a, st);
-    if (vecs <= 64 * 8) return launch<D, 64, 8, 64, kBoth>(a, st);
-    if (vecs <= 64 * 16) return launch<D, 64, 16, 64, kBoth>(a, st);
+    if (waves) {
+        if (vecs <= 64 * 4) return launch<D, 64, 4, 64, kBoth>(a, st);
+        if (vecs <= 64 * 8) return launch<D, 64, 8, 64, kBoth>(a, st);
+    } else {
+        if (vecs <= 256) return launch<D, 256, 1, 64, kBoth>(a, st);
+        if (vecs <= 256 * 2) return launch<D, 256, 2, 64, kBoth>(a, st);
+    }
+    if (vecs <= 256 * 4) return launch<D, 256, 4, 64, kBoth>(a, st);
     if (vecs <= 256 * 8) return launch<D, 256, 8, 64, kBoth>(a, st);
     if (vecs <= 256 * 16) return launch<D, 256, 16, 64, kBoth>(a, st);
     if (vecs <= 1024 * 8) return launch<D, 1024, 8, 64, kBoth>(a, st);
