@@ -78,7 +78,7 @@ struct Vec {
     static constexpr int E = 16 / sizeof(T);
     uint32_t w[4];
     __device__ __forceinline__ void load(const T *at) { __builtin_memcpy(w, at, 16); }
-    __device__ __forceinline__ void store(T *at) const { __builtin_memcpy(at, w, 16); }
+    __device__ __forceinline__ void store(T *at) const { stream16(at, (i32x4){(int)w[0], (int)w[1], (int)w[2], (int)w[3]}); }
     __device__ __forceinline__ float get(int i) const {
         if (sizeof(T) == 4) return __uint_as_float(w[i]);
         const uint16_t h = (uint16_t)(w[i / 2] >> (16 * (i & 1)));

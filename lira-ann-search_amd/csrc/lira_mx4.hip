@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void k_mx4_dequantize(const uint8_t *__restric
     const int64_t j = p * kPlane + lane * E;
     T *q = out + row * ld + j;
     if (VEC && j + E <= k) {
-        *reinterpret_cast<V *>(q) = o;
+        stream16(q, *reinterpret_cast<const i32x4 *>(&o));
     } else {
 #pragma unroll
         for (int i = 0; i < E; ++i)
@@ -221,17 +221,18 @@ __global__ __launch_bounds__(WN *WM *WK * 64) void k_mx4_tile(Product P, int til
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wn = w % WN, wm = w / WN % WM, wk = w / (WN * WM);
 
-    // Workgroups go to the 8 XCDs in turn: each XCD takes a run of tiles of its own, 8 tiles of rows
-    // by as many of columns, so that the tiles in flight on it share their operands in its L2.
+    // Workgroups go to the 8 XCDs in turn: each XCD takes a run of tiles of its own, 4 tiles of rows
+    // high, so that the tiles in flight on it share their operands in its L2 (8192^3, us: 328; 8 high 333;
+    // in launch order 341).
     const int64_t tiles = (int64_t)tiles_n * tiles_m;
     int64_t t = blockIdx.x;
     {
         const int64_t per = tiles / 8, rest = tiles % 8, x = t % 8;
         t = x * per + (x < rest ? x : rest) + t / 8;
     }
-    const int64_t band = t / (8 * (int64_t)tiles_n), in = t % (8 * (int64_t)tiles_n);
-    const int hb = (int)min((int64_t)8, tiles_m - band * 8);
-    const int64_t m0 = (band * 8 + in % hb) * TM, n0 = in / hb * TN;
+    const int64_t band = t / (4 * (int64_t)tiles_n), in = t % (4 * (int64_t)tiles_n);
+    const int hb = (int)min((int64_t)4, tiles_m - band * 4);
+    const int64_t m0 = (band * 4 + in % hb) * TM, n0 = in / hb * TN;
 
     const uint32_t lds = (uint32_t)(uintptr_t)smem;
     const uint8_t *cb = P.bc + n0 * 64, *ca = P.ac + m0 * 64, *sb = P.bs + n0 * 4, *sa = P.as + m0 * 4;
@@ -378,17 +379,14 @@ __global__ __launch_bounds__(WN *WM *WK * 64) void k_mx4_tile(Product P, int til
             const int at = u * 64 + lane, rr = at / (TNw / E), c = at % (TNw / E) * E;
             const int64_t row = row0 + j * 16 + rr, col = col0 + c;
             if (at < kUnits && row < P.m && col < P.n) {
-                struct alignas(16) V {
-                    T e[E];
-                };
-                const V v = *reinterpret_cast<const V *>(stage + rr * kRow + c);
+                const T *v = stage + rr * kRow + c;
                 T *o = (T *)P.out + row * P.ldo + col;
                 if (col + E <= P.n) {
-                    __builtin_memcpy(o, &v, 16);  // (at any alignment)
+                    stream16(o, *reinterpret_cast<const i32x4 *>(v));
                 } else {
 #pragma unroll
                     for (int e = 0; e < E; ++e)
-                        if (col + e < P.n) o[e] = v.e[e];
+                        if (col + e < P.n) o[e] = v[e];
                 }
             }
         }

@@ -18,6 +18,13 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
+// 16 bytes to memory at any alignment, past the caches' write-back (nt): results are whole runs that this
+// kernel does not read again.  8192 x 8192 fp32 out of a 512-deep product 103 us with plain stores, 75 so.
+__device__ __forceinline__ void stream16(void *at, i32x4 v) {
+    typedef int anywhere __attribute__((ext_vector_type(4), aligned(2)));
+    __builtin_nontemporal_store((anywhere)v, (anywhere *)at);
+}
+
 // element types of lira_hip.h's LIRA_DTYPE_*
 struct F32 {
     typedef float T;
