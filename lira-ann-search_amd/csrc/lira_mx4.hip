@@ -13,7 +13,7 @@ static constexpr int kPlane = 128;  // elements per plane
 // ------------------------------------------------------------ pack / unpack
 // 16 lanes per (row, plane), 8 elements each; the block's largest magnitude crosses its 4
 // lanes by DPP.  A wave packs 4 consecutive rows: 256 bytes of codes and 16 of scales.
-template <class D, bool VEC>
+template <class D, bool VEC, bool ONCE>
 __global__ __launch_bounds__(256) void k_mx4_quantize(const typename D::T *__restrict__ x, int64_t n, int64_t k,
                                                       int64_t ld, uint8_t *__restrict__ codes,
                                                       uint8_t *__restrict__ scales, int64_t plane_rows) {
@@ -22,7 +22,7 @@ __global__ __launch_bounds__(256) void k_mx4_quantize(const typename D::T *__res
     const int64_t p = blockIdx.y;
     const bool live = row < n;
     float v[8];
-    load_run<D, VEC, 8>(x + (live ? row : 0) * ld, p * kPlane + lane * 8, k, v);
+    load_run<D, VEC, 8, ONCE>(x + (live ? row : 0) * ld, p * kPlane + lane * 8, k, v);
     const uint32_t s = scale_code(quad_max(v));
     const uint32_t c = s == 255 ? 0u : to_codes(v, scale_operand(s));
     if (!live) return;
@@ -527,11 +527,18 @@ static int quantize(const void *x, int64_t n, int64_t k, int64_t ld, uint8_t *co
     typedef typename D::T T;
     const bool vec = ((uintptr_t)x & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
     const dim3 g((unsigned)((n + 15) / 16), (unsigned)planes_of(k));
-    if (vec)
-        hipLaunchKernelGGL((k_mx4_quantize<D, true>), g, dim3(256), 0, st, (const T *)x, n, k, ld, codes, scales,
+    // What the last kernel left of x may be in the caches; of x several times their size nothing is, and its
+    // loads would push out the packed rows (1M x 128, packed and read back: 196 us, 184 with ONCE;
+    // 10000 x 128 packed 2.9 us, 3.7 with it).
+    const bool once = n * k * (int64_t)sizeof(T) >= (int64_t)128 << 20;
+    if (!vec)
+        hipLaunchKernelGGL((k_mx4_quantize<D, false, false>), g, dim3(256), 0, st, (const T *)x, n, k, ld, codes, scales,
+                           plane_rows);
+    else if (once)
+        hipLaunchKernelGGL((k_mx4_quantize<D, true, true>), g, dim3(256), 0, st, (const T *)x, n, k, ld, codes, scales,
                            plane_rows);
     else
-        hipLaunchKernelGGL((k_mx4_quantize<D, false>), g, dim3(256), 0, st, (const T *)x, n, k, ld, codes, scales,
+        hipLaunchKernelGGL((k_mx4_quantize<D, true, false>), g, dim3(256), 0, st, (const T *)x, n, k, ld, codes, scales,
                            plane_rows);
     LIRA_HIP_TRY(hipGetLastError());
     return LIRA_OK;

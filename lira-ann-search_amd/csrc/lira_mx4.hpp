@@ -94,8 +94,8 @@ __device__ __forceinline__ void from_codes(uint32_t c, uint32_t s, float (&v)[N]
 
 // N = 8 or 32 consecutive elements of a row from element j (zeros past the row's end); VEC: the row's
 // first element and the row stride are multiples of 16 bytes.  The ends of rows read their last
-// element's place again: a branch round every load would wait for each.
-template <class D, bool VEC, int N>
+// element's place again: a branch round every load would wait for each.  ONCE: not kept in the L2.
+template <class D, bool VEC, int N, bool ONCE = false>
 __device__ __forceinline__ void load_run(const typename D::T *row, int64_t j, int64_t k, float (&v)[N]) {
     typedef typename D::T T;
     if (VEC && j + N <= k) {
@@ -104,7 +104,11 @@ __device__ __forceinline__ void load_run(const typename D::T *row, int64_t j, in
             T e[E];
         } t[N / E];
 #pragma unroll
-        for (int i = 0; i < N / E; ++i) t[i] = *reinterpret_cast<const V *>(row + j + i * E);
+        for (int i = 0; i < N / E; ++i) {
+            const i32x4 *at = reinterpret_cast<const i32x4 *>(row + j + i * E);
+            const i32x4 q = ONCE ? __builtin_nontemporal_load(at) : *at;
+            __builtin_memcpy(&t[i], &q, 16);
+        }
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = D::up(t[i / E].e[i % E]);
     } else {
