@@ -168,12 +168,6 @@ def run(name: str, *args) -> None:
         check(rc, name)
 
 
-def raw_stream(device_index: int) -> int:
-    """The current stream of a device as an address, without a torch.cuda.Stream object for it (3 us)."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(device_index)
-
-
 def ptr(t) -> int:
     """Device/host pointer of a torch tensor (or None -> NULL)."""
     if t is None:

@@ -20,7 +20,7 @@ import functools
 import torch
 
 from . import _lib
-from .mx4 import DTYPES, check_rows, on, _rows
+from .mx4 import DTYPES, check_rows, on, raw_stream, _rows
 
 
 def check_device(logits) -> None:
@@ -98,7 +98,7 @@ def _forward(head, dev, stats, row_weight, dz):
     need = _workspace_size(rows, vocab, head[8], head[1])
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _lib.run("lira_distill_topk", *head, loss.data_ptr(), _lib.ptr(stats), _lib.ptr(row_weight), 1, _lib.ptr(dz), vocab,
-             _lib.ptr(ws), need, _lib.raw_stream(dev.index))
+             _lib.ptr(ws), need, raw_stream(dev.index))
     return loss
 
 
@@ -116,7 +116,7 @@ class _Loss(torch.autograd.Function):
             return loss
         out = torch.empty(2, dtype=torch.float32, device=dev)
         _lib.run("lira_distill_reduce", loss.data_ptr(), stats.data_ptr(), head[2], reduction == "mean", out.data_ptr(),
-                 _lib.raw_stream(dev.index))
+                 raw_stream(dev.index))
         ctx.factor = out[1]
         return out[0].clone()
 
@@ -135,7 +135,7 @@ class _Loss(torch.autograd.Function):
                 g = g.contiguous()
             dz = torch.empty((rows, vocab), dtype=z.dtype, device=dev)
             _lib.run("lira_distill_topk_backward", *head, stats.data_ptr(), g.data_ptr(), 0 if whole else 1,
-                     dz.data_ptr(), vocab, _lib.raw_stream(dev.index))
+                     dz.data_ptr(), vocab, raw_stream(dev.index))
         return dz, None, None, None, None, None
 
 

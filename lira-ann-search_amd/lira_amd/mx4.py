@@ -27,6 +27,8 @@ DTYPES = {torch.float32: _lib.LIRA_DTYPE_F32, torch.bfloat16: _lib.LIRA_DTYPE_BF
 ACTIVATIONS = {None: _lib.LIRA_ACT_NONE, "relu": _lib.LIRA_ACT_RELU, "sigmoid": _lib.LIRA_ACT_SIGMOID}
 
 
+# the current stream of a device as an address, without a torch.cuda.Stream object for it (3 us a call)
+raw_stream = torch._C._cuda_getCurrentRawStream
 _HERE = contextlib.nullcontext()
 
 
@@ -148,7 +150,7 @@ def mx4_quantize(x: torch.Tensor, stream=None) -> MX4Tensor:
         codes = torch.empty((p, n, 64), dtype=torch.uint8, device=dev)
         scales = torch.empty((p, n, 4), dtype=torch.uint8, device=dev)
         _lib.run("lira_mx4_quantize", x.data_ptr(), DTYPES[x.dtype], n, k, ld, codes.data_ptr(), scales.data_ptr(), n,
-                 _lib.raw_stream(dev.index))
+                 raw_stream(dev.index))
     return MX4Tensor._made(codes, scales, k)
 
 
@@ -186,7 +188,7 @@ def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float32, out: torch.
     with on(dev, stream):
         out, ld = _out(out, (n, t.k), dtype, dev, t.codes, t.scales)
         _lib.run("lira_mx4_dequantize", t.codes.data_ptr(), t.scales.data_ptr(), t.plane_rows, n, t.k, out.data_ptr(),
-                 DTYPES[dtype], ld, _lib.raw_stream(dev.index))
+                 DTYPES[dtype], ld, raw_stream(dev.index))
     return out
 
 
@@ -223,7 +225,7 @@ def mx4_matmul(a: MX4Tensor, b: MX4Tensor, bias: torch.Tensor | None = None, act
         out, ldo = _out(out, (m, n), out_dtype, dev, a.codes, a.scales, b.codes, b.scales, bias)
         _lib.run("lira_mx4_matmul", a.codes.data_ptr(), a.scales.data_ptr(), a.plane_rows, m, b.codes.data_ptr(),
                  b.scales.data_ptr(), b.plane_rows, n, a.k, alpha, _lib.ptr(bias), act, out.data_ptr(),
-                 DTYPES[out_dtype], ldo, _lib.raw_stream(dev.index))
+                 DTYPES[out_dtype], ldo, raw_stream(dev.index))
     return out
 
 
@@ -256,5 +258,5 @@ def mx4_linear(x: torch.Tensor, w: MX4Tensor, bias: torch.Tensor | None = None, 
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.run("lira_mx4_linear", x.data_ptr(), DTYPES[x.dtype], m, k, ld, w.codes.data_ptr(), w.scales.data_ptr(),
                  w.plane_rows, n, alpha, _lib.ptr(bias), act, out.data_ptr(), DTYPES[out_dtype], ldo, _lib.ptr(ws), need,
-                 _lib.raw_stream(dev.index))
+                 raw_stream(dev.index))
     return out
