@@ -32,13 +32,11 @@ def _rows_of(t: torch.Tensor) -> torch.Tensor:
     return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
 
 
-def _fp32(t):
-    """A constant of the kernels: detached, float32, contiguous (None stays None)."""
-    if t is None:
-        return None
+def _fp32(t: torch.Tensor) -> torch.Tensor:
+    """A constant of the kernels: detached, float32, contiguous."""
     if t.requires_grad:
         t = t.detach()
-    return t.to(torch.float32).contiguous()
+    return (t if t.dtype == torch.float32 else t.to(torch.float32)).contiguous()
 
 
 def _row_values(t, name: str, lead, device):
@@ -46,30 +44,27 @@ def _row_values(t, name: str, lead, device):
         return None
     if not isinstance(t, torch.Tensor) or t.device != device or t.shape != lead or not t.is_floating_point():
         raise ValueError(f"{name} must be a {tuple(lead)} float tensor on {device}")
-    return _fp32(t.reshape(-1))
+    return _fp32(t if len(lead) == 1 else t.reshape(-1))
 
 
 def _entries(logits, top_ids, top_logits, temperature, teacher_lse):
     """(logits (rows, vocab), the logits' leading dimensions, ids, teacher's logits, its logsumexp), checked and as
     the kernels read them (the teacher is constant)."""
-    check_device(logits)
     shape, dev = logits.shape, logits.device
-    if not shape:
-        raise ValueError("logits must have at least one dimension")
-    lead, vocab = shape[:-1], shape[-1]
-    if vocab < 1:
-        raise ValueError("logits must have at least one output")
+    if not shape or not shape[-1]:
+        raise ValueError("logits must have at least one dimension and one output")
+    lead = shape[:-1]
     z = check_rows(_rows_of(logits), "logits")
     for t, name in ((top_ids, "top_ids"), (top_logits, "top_logits")):
         if not isinstance(t, torch.Tensor) or t.device != dev:
             raise ValueError(f"{name} must be a tensor on {dev}")
-        if t.shape[:-1] != lead or t.dim() != logits.dim():
+        if t.dim() != len(shape) or t.shape[:-1] != lead:
             raise ValueError(f"{name} must have the logits' leading dimensions {tuple(lead)}, not {tuple(t.shape[:-1])}")
-    if top_ids.dtype != torch.int32 and top_ids.dtype != torch.int64:
+    if top_ids.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"top_ids must be int32 or int64, not {top_ids.dtype}")
     if top_logits.dtype not in DTYPES:
         raise ValueError(f"top_logits must be float32, bfloat16 or float16, not {top_logits.dtype}")
-    if top_ids.shape[-1] < 1 or top_logits.shape != top_ids.shape:
+    if top_logits.shape != top_ids.shape or not top_ids.shape[-1]:
         raise ValueError(f"top_ids {tuple(top_ids.shape)} and top_logits {tuple(top_logits.shape)} must have the same "
                          "shape, at least one entry a row")
     if not 0.0 < temperature < float("inf"):
@@ -107,11 +102,11 @@ class _Loss(torch.autograd.Function):
     def forward(ctx, z, ids, tv, lse, t, reduction):
         dev = z.device
         z = _rows(z)[0]
-        ctx.head = head = _head(z, ids, tv, lse, t)
+        head = _head(z, ids, tv, lse, t)
         stats = torch.empty((head[2], 4), dtype=torch.float32, device=dev)
         loss = _forward(head, dev, stats, None, None)
-        ctx.save_for_backward(z, ids, tv, lse, stats)  # (what the head points to, kept and checked for changes)
-        ctx.factor = None
+        ctx.save_for_backward(z, ids, tv, lse, stats)
+        ctx.t, ctx.factor = t, None
         if reduction == "none":
             return loss
         out = torch.empty(2, dtype=torch.float32, device=dev)
@@ -124,8 +119,9 @@ class _Loss(torch.autograd.Function):
     def backward(ctx, g):
         if torch.is_grad_enabled():
             raise RuntimeError("distill_topk_loss has no second derivative (create_graph=True)")
-        z, _, _, _, stats = ctx.saved_tensors
-        head, dev = ctx.head, z.device
+        z, ids, tv, lse, stats = ctx.saved_tensors  # (not always the tensors of the forward pass: hooks may have moved them)
+        z, dev = _rows(z)[0], z.device
+        head = _head(z, ids, tv, lse, ctx.t)
         rows, vocab = head[2], head[3]
         with on(dev):
             if ctx.factor is not None:
@@ -160,7 +156,6 @@ def distill_topk_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_logits: t
     return loss.view(lead) if reduction == "none" and len(lead) != 1 else loss
 
 
-@torch.no_grad()
 def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_logits: torch.Tensor,
                                temperature: float = 1.0, teacher_lse: torch.Tensor | None = None,
                                row_weight: torch.Tensor | None = None, grad_out: torch.Tensor | None = None,

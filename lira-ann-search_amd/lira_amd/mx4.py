@@ -75,30 +75,51 @@ class MX4Tensor:
     """Packed rows: ``codes`` (P, n, 64) uint8, ``scales`` (P, n, 4) uint8, P = ceil(k / 128)
     planes of 128 elements (include/lira_hip.h).  Row ranges ``t[lo:hi]`` are views."""
 
-    __slots__ = ("codes", "scales", "k", "plane_rows")
+    # (what mx4_quantize packs is one buffer, whose two views are made when they are asked for)
+    __slots__ = ("_codes", "_scales", "_buf", "k", "n", "plane_rows", "device", "codes_ptr", "scales_ptr")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int):
         k = int(k)
         for t, w, name in ((codes, 64, "codes"), (scales, 4, "scales")):
             if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 3 or t.shape[2] != w:
                 raise ValueError(f"{name} must be a (P, n, {w}) uint8 tensor on the GPU")
-        if k < 1 or codes.shape[0] != (k + 127) // 128:
-            raise ValueError(f"k = {k} needs {(max(k, 1) + 127) // 128} planes, codes have {codes.shape[0]}")
-        if codes.shape[:2] != scales.shape[:2] or codes.device != scales.device:
+        p, n, _ = codes.shape
+        if k < 1 or p != (k + 127) // 128:
+            raise ValueError(f"k = {k} needs {(max(k, 1) + 127) // 128} planes, codes have {p}")
+        if scales.shape[0] != p or scales.shape[1] != n or codes.device != scales.device:
             raise ValueError("codes and scales must have the same planes and rows, on one device")
         rows = self._plane_rows(codes)
         if rows is None or rows != self._plane_rows(scales) or codes.data_ptr() % 16 or scales.data_ptr() % 4:
             codes, scales = codes.clone(memory_format=torch.contiguous_format), \
                 scales.clone(memory_format=torch.contiguous_format)
-            rows = codes.shape[1]
-        self.codes, self.scales, self.k, self.plane_rows = codes, scales, k, rows
+            rows = n
+        self._codes, self._scales, self._buf = codes, scales, None
+        self.k, self.n, self.plane_rows, self.device = k, n, rows, codes.device
+        self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
-    def _made(cls, codes, scales, k) -> "MX4Tensor":
-        """Of two contiguous tensors that this module has just made."""
+    def _of(cls, buf: torch.Tensor, device: torch.device, n: int, k: int) -> "MX4Tensor":
+        """Of one buffer: the codes, then the scales."""
         t = object.__new__(cls)
-        t.codes, t.scales, t.k, t.plane_rows = codes, scales, k, codes.shape[1]
+        t._codes = t._scales = None
+        t._buf, t.k, t.n, t.plane_rows, t.device = buf, k, n, n, device
+        t.codes_ptr = buf.data_ptr()
+        t.scales_ptr = t.codes_ptr + (k + 127) // 128 * n * 64
         return t
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            p = (self.k + 127) // 128
+            self._codes = self._buf[:p * self.n * 64].view(p, self.n, 64)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            p = (self.k + 127) // 128
+            self._scales = self._buf[p * self.n * 64:].view(p, self.n, 4)
+        return self._scales
 
     @staticmethod
     def _plane_rows(t: torch.Tensor):
@@ -113,17 +134,13 @@ class MX4Tensor:
 
     @property
     def shape(self) -> tuple[int, int]:
-        return self.codes.shape[1], self.k
-
-    @property
-    def device(self) -> torch.device:
-        return self.codes.device
+        return self.n, self.k
 
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return (self.k + 127) // 128 * self.n * 68
 
     def __len__(self) -> int:
-        return self.codes.shape[1]
+        return self.n
 
     def __getitem__(self, rows: slice) -> "MX4Tensor":
         if not isinstance(rows, slice) or rows.step not in (None, 1):
@@ -147,11 +164,10 @@ def mx4_quantize(x: torch.Tensor, stream=None) -> MX4Tensor:
     dev = x.device
     with on(dev, stream):
         x, ld = _rows(x)
-        codes = torch.empty((p, n, 64), dtype=torch.uint8, device=dev)
-        scales = torch.empty((p, n, 4), dtype=torch.uint8, device=dev)
-        _lib.run("lira_mx4_quantize", x.data_ptr(), DTYPES[x.dtype], n, k, ld, codes.data_ptr(), scales.data_ptr(), n,
+        t = MX4Tensor._of(torch.empty(p * n * 68, dtype=torch.uint8, device=dev), dev, n, k)
+        _lib.run("lira_mx4_quantize", x.data_ptr(), DTYPES[x.dtype], n, k, ld, t.codes_ptr, t.scales_ptr, n,
                  raw_stream(dev.index))
-    return MX4Tensor._made(codes, scales, k)
+    return t
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -170,8 +186,8 @@ def _out(out, shape, dtype, device, *inputs) -> tuple[torch.Tensor, int]:
     if shape[1] > 1 and out.stride(1) != 1 or shape[0] > 1 and out.stride(0) < shape[1]:
         raise ValueError("out must have rows of consecutive elements that do not overlap")
     lo, hi = _span(out)
-    for t in inputs:
-        if t is not None and lo < _span(t)[1] and _span(t)[0] < hi:
+    for t in (v for i in inputs if i is not None for v in ((i.codes, i.scales) if isinstance(i, MX4Tensor) else (i,))):
+        if lo < _span(t)[1] and _span(t)[0] < hi:
             raise ValueError("out must not share memory with an input")
     _no_grad(out)
     return out, out.stride(0) if shape[0] > 1 else max(1, shape[1])
@@ -184,11 +200,11 @@ def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float32, out: torch.
         raise ValueError("t must be an MX4Tensor")
     if dtype not in DTYPES:
         raise ValueError(f"dtype must be float32, bfloat16 or float16, not {dtype}")
-    dev, n = t.codes.device, t.codes.shape[1]
+    dev, n = t.device, t.n
     with on(dev, stream):
-        out, ld = _out(out, (n, t.k), dtype, dev, t.codes, t.scales)
-        _lib.run("lira_mx4_dequantize", t.codes.data_ptr(), t.scales.data_ptr(), t.plane_rows, n, t.k, out.data_ptr(),
-                 DTYPES[dtype], ld, raw_stream(dev.index))
+        out, ld = _out(out, (n, t.k), dtype, dev, t)
+        _lib.run("lira_mx4_dequantize", t.codes_ptr, t.scales_ptr, t.plane_rows, n, t.k, out.data_ptr(), DTYPES[dtype], ld,
+                 raw_stream(dev.index))
     return out
 
 
@@ -199,9 +215,9 @@ def _epilogue(w, bias, activation):
         raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, not {activation!r}")
     if bias is None:
         return None, ACTIVATIONS[activation]
-    if not isinstance(bias, torch.Tensor) or bias.device != w.device or tuple(bias.shape) != (w.shape[0],) \
+    if not isinstance(bias, torch.Tensor) or bias.device != w.device or tuple(bias.shape) != (w.n,) \
             or not bias.is_floating_point():
-        raise ValueError(f"bias must be a ({w.shape[0]},) float tensor on {w.device}")
+        raise ValueError(f"bias must be a ({w.n},) float tensor on {w.device}")
     _no_grad(bias)
     return bias, ACTIVATIONS[activation]
 
@@ -218,13 +234,12 @@ def mx4_matmul(a: MX4Tensor, b: MX4Tensor, bias: torch.Tensor | None = None, act
         raise ValueError(f"a has {a.k} columns on {a.device}, b has {b.k} on {b.device}")
     if out_dtype not in DTYPES:
         raise ValueError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
-    m, n = a.shape[0], b.shape[0]
+    m, n = a.n, b.n
     dev = a.device
     with on(dev, stream):
         bias = None if bias is None else bias.to(torch.float32).contiguous()
-        out, ldo = _out(out, (m, n), out_dtype, dev, a.codes, a.scales, b.codes, b.scales, bias)
-        _lib.run("lira_mx4_matmul", a.codes.data_ptr(), a.scales.data_ptr(), a.plane_rows, m, b.codes.data_ptr(),
-                 b.scales.data_ptr(), b.plane_rows, n, a.k, alpha, _lib.ptr(bias), act, out.data_ptr(),
+        out, ldo = _out(out, (m, n), out_dtype, dev, a, b, bias)
+        _lib.run("lira_mx4_matmul", a.codes_ptr, a.scales_ptr, a.plane_rows, m, b.codes_ptr, b.scales_ptr, b.plane_rows, n, a.k, alpha, _lib.ptr(bias), act, out.data_ptr(),
                  DTYPES[out_dtype], ldo, raw_stream(dev.index))
     return out
 
@@ -249,14 +264,13 @@ def mx4_linear(x: torch.Tensor, w: MX4Tensor, bias: torch.Tensor | None = None, 
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if out_dtype not in DTYPES:
         raise ValueError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
-    m, n, k, dev = x.shape[0], w.codes.shape[1], w.k, x.device
+    m, n, k, dev = x.shape[0], w.n, w.k, x.device
     need = _linear_workspace(m, n, k)
     with on(dev, stream):
         x, ld = _rows(x)
         bias = None if bias is None else bias.to(torch.float32).contiguous()
-        out, ldo = _out(out, (m, n), out_dtype, dev, x, w.codes, w.scales, bias)
+        out, ldo = _out(out, (m, n), out_dtype, dev, x, w, bias)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _lib.run("lira_mx4_linear", x.data_ptr(), DTYPES[x.dtype], m, k, ld, w.codes.data_ptr(), w.scales.data_ptr(),
-                 w.plane_rows, n, alpha, _lib.ptr(bias), act, out.data_ptr(), DTYPES[out_dtype], ldo, _lib.ptr(ws), need,
+        _lib.run("lira_mx4_linear", x.data_ptr(), DTYPES[x.dtype], m, k, ld, w.codes_ptr, w.scales_ptr, w.plane_rows, n, alpha, _lib.ptr(bias), act, out.data_ptr(), DTYPES[out_dtype], ldo, _lib.ptr(ws), need,
                  raw_stream(dev.index))
     return out

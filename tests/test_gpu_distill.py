@@ -116,6 +116,19 @@ def test_no_second_derivative():
         loss.backward()
 
 
+def test_tensors_saved_elsewhere():
+    """The backward pass on what the hooks bring back (offloaded activations), not on the first addresses."""
+    from lira_amd import distill_topk_loss
+    z, ti, tv, w = make(40, 3000, 9, "bf16")
+    z.requires_grad_(True)
+    (want,) = torch.autograd.grad(distill_topk_loss(z, ti, tv, 2.0, reduction="none"), z, w)
+    with torch.autograd.graph.save_on_cpu():
+        loss = distill_topk_loss(z * 1.0, ti.clone(), tv.clone(), 2.0, reduction="none")
+    junk = [torch.full_like(x, 7) for x in (z.detach(), ti, tv) for _ in range(4)]  # (over what was freed)
+    (got,) = torch.autograd.grad(loss, z, w)
+    assert torch.equal(got, want) and len(junk) == 12
+
+
 def test_no_row_counts():
     from lira_amd import distill_topk_loss
     z, ti, tv, _ = make(5, 70, 4)

@@ -78,6 +78,25 @@ def test_pack_ties_and_extremes():
     assert not t.codes[0, 7, :48].any()  # (codes of a NaN block are 0)
 
 
+def test_views_of_a_packed_tensor():
+    from lira_amd import MX4Tensor, mx4_linear, mx4_quantize
+    x = torch.randn(50, 300, generator=gen(4), device="cuda")
+    t = mx4_quantize(x)
+    assert t.codes.shape == (3, 50, 64) and t.scales.shape == (3, 50, 4) and t.nbytes() == 3 * 50 * 68 and len(t) == 50
+    assert t.codes.data_ptr() == t.codes_ptr and t.scales.data_ptr() == t.scales_ptr and t.device == x.device
+    want, _ = ref_pack(x)
+    same(MX4Tensor(t.codes, t.scales, 300).dequantize(), want)
+    same(t[10:10].dequantize(), want[10:10])
+    same(t[49:].dequantize(), want[49:])
+    same(t[5:40][3:4].dequantize(), want[8:9])
+    # parts whose rows are spaced differently, or that lie apart, are brought together
+    wide = torch.zeros(3, 50, 80, dtype=torch.uint8, device="cuda")
+    wide[..., 16:] = t.codes
+    same(MX4Tensor(wide[..., 16:], t.scales, 300).dequantize(), want)
+    q = torch.randn(3, 300, generator=gen(5), device="cuda")
+    assert torch.equal(mx4_linear(q, t[7:30]), mx4_linear(q, mx4_quantize(x[7:30])))
+
+
 def every_code():
     """All 16 codes under all 256 scales: (256, 128) packed rows and their values in 64 bits."""
     codes = torch.zeros(1, 256, 64, dtype=torch.uint8)
