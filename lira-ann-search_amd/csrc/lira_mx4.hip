@@ -74,6 +74,7 @@ struct Epilogue {
     const float *bias;
     float alpha;
     int act;
+    bool bias16;  // whole runs of 4: aligned, and n a multiple of 4
 };
 // alpha acc + bias and the activation, in place
 template <int N>
@@ -99,7 +100,9 @@ __device__ __forceinline__ void finish(f32x4 (&acc)[N], f32x4 bias, const Epilog
 // 4 columns of the bias, 0 where there is none (past the end the last one's: not stored)
 __device__ __forceinline__ f32x4 bias4(const Epilogue &e, int64_t col, int64_t n) {
     f32x4 b = {0, 0, 0, 0};
-    if (e.bias) {
+    if (e.bias16) {
+        b = *reinterpret_cast<const f32x4 *>(e.bias + min(col, n - 4));
+    } else if (e.bias) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) b[i] = e.bias[min(col + i, n - 1)];
     }
@@ -396,9 +399,8 @@ __global__ __launch_bounds__(WN *WM *WK * 64) void k_mx4_tile(Product P, int til
 
 // The few-rows kernel: 16 NB columns of the output x up to 16 rows, a stream over W.  No operand is
 // shared between waves, so W goes straight to registers: a wave's load of a fragment is 1 KiB in a row.
-// KS waves of a workgroup split the planes and join their sums in LDS in a fixed order.  KS = 1, where
-// there are few planes: four waves, each of its own columns, and workgroups that go on to the next
-// columns, whose first plane is on its way while the last one is finished.  FUSED: the rows of x are
+// KS waves of a workgroup split the planes and join their sums in LDS in a fixed order.  KS = 1, where there are
+// few planes or many columns: four waves, each of its own columns, that go on to the next ones without a gap.  FUSED: the rows of x are
 // packed here, 32 elements a thread, while the first planes of W are on their way; else they come
 // packed and are read from the cache.
 struct Rows {
@@ -407,7 +409,7 @@ struct Rows {
 };
 template <class X, class D, int NB, int KS, bool FUSED, bool VEC>
 __global__ __launch_bounds__(KS == 1 ? 256 : KS * 64, 4) void k_mx4_rows(Product P, Rows R) {
-    constexpr int U = KS == 1 ? 1 : FUSED ? 3 : 4;  // planes in flight
+    constexpr int U = KS == 1 ? 2 : FUSED ? 3 : 4;  // planes in flight
     constexpr int NT = KS == 1 ? 256 : KS * 64;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -420,6 +422,7 @@ __global__ __launch_bounds__(KS == 1 ? 256 : KS * 64, 4) void k_mx4_rows(Product
     struct Step {
         i32x4 b[NB], a;
         int sb[NB], sa;
+        f32x4 bias[NB];  // (KS = 1, with a group's last plane: a load of its own would wait for those ahead of it)
     } f[U];
     const int stride = FUSED ? planes * 64 + 16 : 0;  // of a packed row in LDS (its banks turn by 4)
     uint8_t *xs = smem + (FUSED ? m * stride : 0);
@@ -433,14 +436,28 @@ __global__ __launch_bounds__(KS == 1 ? 256 : KS * 64, 4) void k_mx4_rows(Product
             q.b[i] = __builtin_nontemporal_load(reinterpret_cast<const i32x4 *>(c + at * 16));
             q.sb[i] = s[at];
         }
+        if (KS == 1 && p == planes - 1) {
+#pragma unroll
+            for (int i = 0; i < NB; ++i) q.bias[i] = bias4(P.ep, row + i * 16 + g * 4, P.n);
+        }
         if (!FUSED) {
             q.a = *reinterpret_cast<const i32x4 *>(P.ac + p * aplane + ao * 64 + g * 16);
             q.sa = P.as[p * (aplane >> 4) + ao * 4 + g];
         }
     };
-    if (KS > 1 || group < groups) {
+    // KS = 1: one run of planes, group after group; the loads are U planes ahead of the products
+    int64_t ahead = group;
+    int plane_ahead = 0;
+    auto load_next = [&](Step &q) {
+        if (ahead < groups) load(q, ahead, plane_ahead);
+        if (++plane_ahead == planes) plane_ahead = 0, ahead += step;
+    };
 #pragma unroll
-        for (int u = 0; u < U; ++u) load(f[u], group, min(first + u * KS, planes - 1));
+    for (int u = 0; u < U; ++u) {
+        if (KS == 1)
+            load_next(f[u]);
+        else
+            load(f[u], group, min(first + u * KS, planes - 1));
     }
     if (FUSED) {
         // 8 elements a thread, the blocks' largest by DPP as in k_mx4_quantize
@@ -461,51 +478,66 @@ __global__ __launch_bounds__(KS == 1 ? 256 : KS * 64, 4) void k_mx4_rows(Product
         finish(t, bias, P.ep);
         store_run<D>((typename D::T *)P.out + r * P.ldo + col, t[0], P.n - col);
     };
-    for (; group < groups; group += step) {
-        f32x4 acc[NB], bias[NB];
+    auto packed = [&](Step &q, int p) {
+        q.a = *reinterpret_cast<const i32x4 *>(smem + ao * stride + p * 64 + g * 16);
+        q.sa = xs[ao * planes * 4 + p * 4 + g];
+    };
+    f32x4 acc[NB];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            acc[i] = (f32x4){0, 0, 0, 0};
-            if (KS == 1) bias[i] = bias4(P.ep, group * (16 * NB) + i * 16 + g * 4, P.n);
-        }
-        for (int p = first; p < planes; p += U * KS) {
+    for (int i = 0; i < NB; ++i) acc[i] = (f32x4){0, 0, 0, 0};
+    auto multiply = [&](const Step &q) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) acc[i] = mfma(q.b[i], q.sb[i], q.a, q.sa, acc[i]);
+    };
+    if (KS == 1) {
+        int p = 0;
+        while (group < groups) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (p + u * KS >= planes) break;  // (the whole wave)
-                if (FUSED) {
-                    f[u].a = *reinterpret_cast<const i32x4 *>(smem + ao * stride + (p + u * KS) * 64 + g * 16);
-                    f[u].sa = xs[ao * planes * 4 + (p + u * KS) * 4 + g];
-                }
+                if (group >= groups) break;  // (the whole wave)
+                if (FUSED) packed(f[u], p);
+                multiply(f[u]);
+                if (++p == planes) {
 #pragma unroll
-                for (int i = 0; i < NB; ++i) acc[i] = mfma(f[u].b[i], f[u].sb[i], f[u].a, f[u].sa, acc[i]);
-                const int next = p + (U + u) * KS;
-                if (next < planes)
-                    load(f[u], group, next);
-                else if (KS == 1 && group + step < groups)
-                    load(f[u], group + step, 0);
+                    for (int i = 0; i < NB; ++i) {
+                        store(acc[i], f[u].bias[i], group * (16 * NB) + i * 16 + g * 4);
+                        acc[i] = (f32x4){0, 0, 0, 0};
+                    }
+                    p = 0;
+                    group += step;
+                }
+                load_next(f[u]);
             }
         }
-        if (KS == 1) {
+        return;
+    }
+    for (int p = first; p < planes; p += U * KS) {
 #pragma unroll
-            for (int i = 0; i < NB; ++i) store(acc[i], bias[i], group * (16 * NB) + i * 16 + g * 4);
-            continue;
+        for (int u = 0; u < U; ++u) {
+            if (p + u * KS >= planes) break;  // (the whole wave)
+            if (FUSED) packed(f[u], p + u * KS);
+            multiply(f[u]);
+            if (p + (U + u) * KS < planes) load(f[u], group, p + (U + u) * KS);
         }
-        __syncthreads();  // (the packed rows are no longer read)
-        f32x4 *red = reinterpret_cast<f32x4 *>(smem);
+    }
+    __syncthreads();  // (the packed rows are no longer read)
+    f32x4 *red = reinterpret_cast<f32x4 *>(smem);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) red[(i * KS + w) * 64 + lane] = acc[i];
-        __syncthreads();
-        for (int t = w; t < NB; t += KS) {
-            f32x4 y = red[t * KS * 64 + lane];
+    for (int i = 0; i < NB; ++i) red[(i * KS + w) * 64 + lane] = acc[i];
+    __syncthreads();
+    for (int t = w; t < NB; t += KS) {
+        f32x4 y = red[t * KS * 64 + lane];
 #pragma unroll
-            for (int q = 1; q < KS; ++q) y += red[(t * KS + q) * 64 + lane];
-            const int64_t col = group * (16 * NB) + t * 16 + g * 4;
-            store(y, bias4(P.ep, col, P.n), col);
-        }
+        for (int q = 1; q < KS; ++q) y += red[(t * KS + q) * 64 + lane];
+        const int64_t col = group * (16 * NB) + t * 16 + g * 4;
+        store(y, bias4(P.ep, col, P.n), col);
     }
 }
 
 // ---------------------------------------------------------------- launchers
+static Epilogue epilogue(const float *bias, float alpha, int act, int64_t n) {
+    return {bias, alpha, act, bias && ((uintptr_t)bias & 15) == 0 && n % 4 == 0};
+}
 static bool dtype_ok(int dtype) { return dtype >= LIRA_DTYPE_F32 && dtype <= LIRA_DTYPE_F16; }
 static int64_t planes_of(int64_t k) { return (k + kPlane - 1) / kPlane; }
 static int check_packed(const void *codes, const void *scales, int64_t rows, int64_t plane_rows, int64_t k) {
@@ -585,7 +617,7 @@ static int launch_rows(const Product &p, const Rows &r, hipStream_t st) {
     const int bytes = std::max(KS == 1 ? 0 : KS * NB * 1024, FUSED ? (int)p.m * (p.planes * 68 + 16) : 0);
     LIRA_HIP_TRY(set_smem_attr_once(latch, fn, 65536));
     const int64_t groups = (p.n + 16 * NB - 1) / (16 * NB);
-    // (KS = 1: as many workgroups of 4 waves as the 256 compute units hold, 4 waves a SIMD)
+    // (KS = 1: as many workgroups of 4 waves as the 256 compute units hold, 6 waves a SIMD)
     const int64_t blocks = KS == 1 ? std::min<int64_t>((groups + 3) / 4, 256 * 6) : groups;
     hipLaunchKernelGGL((k_mx4_rows<X, D, NB, KS, FUSED, VEC>), dim3((unsigned)blocks), dim3(KS == 1 ? 256 : KS * 64), bytes, st,
                        p, r);
@@ -596,10 +628,14 @@ static int launch_rows(const Product &p, const Rows &r, hipStream_t st) {
 static constexpr int64_t kFusedMax = 4;
 static bool fused_rows(int64_t m, int64_t k) { return m <= kFusedMax && m * (planes_of(k) * 68 + 16) <= 49152; }
 
+// 4096 tiles of 16 columns are enough loads in flight without the planes split (one row, us split and not: 32768 x
+// 4096 18 and 26, 65536 x 4096 32 and 25, 200000 x 900 54 and 19).
+static bool split_planes(const Product &p) { return p.planes >= 8 && (p.n + 15) / 16 < 4096; }
+
 template <class X, class D>
 static int linear_rows(const Product &p, const Rows &r, hipStream_t st) {
     const bool vec = ((uintptr_t)r.x & 15) == 0 && (r.ldx * sizeof(typename X::T)) % 16 == 0;
-    if (p.planes >= 8)
+    if (split_planes(p))
         return vec ? launch_rows<X, D, 1, 8, true, true>(p, r, st) : launch_rows<X, D, 1, 8, true, false>(p, r, st);
     return vec ? launch_rows<X, D, 2, 1, true, true>(p, r, st) : launch_rows<X, D, 2, 1, true, false>(p, r, st);
 }
@@ -613,7 +649,7 @@ template <class D>
 static int product(const Product &p, hipStream_t st) {
     if (p.m <= 16) {
         const Rows r = {nullptr, 0, 0};
-        if (p.planes >= 8) return launch_rows<F32, D, 1, 8, false, false>(p, r, st);
+        if (split_planes(p)) return launch_rows<F32, D, 1, 8, false, false>(p, r, st);
         return launch_rows<F32, D, 2, 1, false, false>(p, r, st);
     }
     // Rows alone decide while one tile takes them all; then the largest tile that still gives each of
@@ -686,7 +722,7 @@ int lira_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, int64_t a_p
     if (m == 0 || n == 0) return LIRA_OK;
     hipStream_t st = (hipStream_t)stream;
     const Product p = {a_codes, a_scales, b_codes, b_scales, a_plane_rows, b_plane_rows, m, n, ldo,
-                       (int)planes_of(k), {bias, alpha, act}, out};
+                       (int)planes_of(k), epilogue(bias, alpha, act, n), out};
     return product(p, out_dtype, st);
 }
 
@@ -713,7 +749,7 @@ int lira_mx4_linear(const void *x, int dtype, int64_t m, int64_t k, int64_t ldx,
         return fail(LIRA_EINVAL, "workspace too small (lira_mx4_linear_workspace_size) or not 16-byte aligned");
     if (!need) {
         const Product p = {nullptr, nullptr, b_codes, b_scales, 0, b_plane_rows, m, n, ldo,
-                           (int)planes_of(k), {bias, alpha, act}, out};
+                           (int)planes_of(k), epilogue(bias, alpha, act, n), out};
         const Rows r = {x, k, ldx};
         if (dtype == LIRA_DTYPE_F32) return linear_rows<F32>(p, r, out_dtype, (hipStream_t)stream);
         if (dtype == LIRA_DTYPE_BF16) return linear_rows<BF16>(p, r, out_dtype, (hipStream_t)stream);
