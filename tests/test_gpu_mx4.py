@@ -170,7 +170,7 @@ def check_product(got, av, bv, alpha, bias, act, dtype):
 SHAPES = [(1, 1, 1), (1, 16, 128), (1, 33, 500), (2, 100, 96), (7, 257, 1000), (15, 64, 129), (16, 31, 256), (17, 130, 384),
           (33, 1000, 960), (64, 64, 64), (65, 65, 4097), (100, 1, 128), (128, 256, 512), (129, 300, 1152), (257, 513, 130),
           (300, 1024, 128), (2100, 2111, 390), (4111, 4113, 260), (1000, 255, 2049), (1, 5000, 128), (3, 4099, 8192), (48, 2000, 3000),
-          (1, 65600, 1100), (3, 70001, 1024), (9, 65537, 1030), (2, 30011, 700), (16, 66000, 100)]  # (columns enough for a loop of groups)
+          (1, 65600, 1100), (3, 70001, 1024), (9, 65537, 1030), (2, 30011, 700), (4, 8200, 4100), (1, 20000, 1100), (16, 66000, 100)]  # (columns enough for a loop of groups)
 
 
 @pytest.mark.parametrize("dtype", list(DT))
