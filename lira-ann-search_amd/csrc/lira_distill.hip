@@ -14,7 +14,11 @@
 //
 // A group of NT threads works on a row (or a slice of it).  Thread u holds the 16-byte vectors u,
 // u + NT, ..: in registers (NV of them) where loss and gradient are wanted together, so that z is
-// read from memory once.  Rows need not be aligned: the vectors are of the row, not of memory.
+// read from memory once.  Rows need not be aligned: the vectors begin where the gradient (the row
+// itself, if only the loss is wanted) is, and up to two vectors' elements at the ends are single
+// (2048 x 131071 bf16, loss and gradient: 251 us, 271 with vectors from the row's first element;
+// the loss alone 99 and 117).  Which thread adds an element, so the last bits of a sum, follows from
+// that alignment.
 //
 // The teacher's entries change single places of the gradient.  The first wave puts each entry
 // into a list of the thread that stores its place (LDS); that thread stores the place once more
@@ -128,7 +132,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
     __shared__ float sm[G][NW], ss[G][NW];
     __shared__ float s_p[G][kEntries ? KM : 1], s_x[G][kEntries ? KM : 1];
     __shared__ int s_id[G][kEntries ? KM : 1], s_next[G][kEntries ? KM : 1], s_head[G][kDz ? NT : 1];
-    __shared__ float s_tot[G][4];
+    __shared__ float s_tot[G][2];
     const int gi = G == 1 ? 0 : threadIdx.x >> 6, u = G == 1 ? threadIdx.x : threadIdx.x & 63;
     const int lane = threadIdx.x & 63, w = G == 1 ? threadIdx.x >> 6 : 0;
     auto sync = [&]() {
@@ -146,14 +150,16 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
     if (r >= a.rows) return;  // (a whole wave, only where groups are waves)
     const T *z = (const T *)a.z + r * a.ldz;
     const float c = kLog2e / a.t;
-    // the slice's vectors [v0, v1) and places [j0, j1)
-    // -- the row's whole vectors; its last vocab % E elements are single, one to each of the last
-    // slice's first threads
-    const int nvec = (int)(a.vocab / E);
+    // the vectors begin h elements in; the slice's are [v0, v1); the elements before the first and behind the
+    // last are single, one to each of the last slice's first threads
+    const uintptr_t from = MODE != kLoss && kDz ? (uintptr_t)((const T *)a.dz + r * a.ldd) : (uintptr_t)z;
+    const int h = min((int)a.vocab, (int)(-from & 15) / (int)sizeof(T));
+    const int nvec = ((int)a.vocab - h) / E, shift = nvec * E;  // (element j + shift is single behind, j >= h)
     const int v0 = a.slices > 1 ? slice * kSliceVecs : 0;
     const int v1 = a.slices > 1 ? min(nvec, v0 + kSliceVecs) : nvec;
-    const int t0 = slice == a.slices - 1 ? nvec * E : (int)a.vocab;  // (vocab: no single ones here)
-    const bool single = u < (int)a.vocab - t0;
+    const int singles = slice == a.slices - 1 ? (int)a.vocab - shift : 0;
+    const bool single = u < singles;
+    const int at1 = u < h ? u : u + shift;
 
     // ------------------------------------------- the entries' loads first
     int id[J];
@@ -176,13 +182,16 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
     float m = -INFINITY, s = 0.0f;
     if (kStats) {
         if (NV) {
-            // (NV / 2 NT < whole vectors <= NV NT: only the later half can be missing; a missing one is
-            // read from the last one's place, which costs less than a branch round every load)
+            // (NV / 2 NT <= vectors <= NV NT: only the later half can be missing; a missing one is read
+            // from the last one's place, which costs less than a branch round every load)
 #pragma unroll
-            for (int i = 0; i < NV; ++i) x[i].load(z + (i < NV / 2 ? i * NT + u : min(i * NT + u, nvec - 1)) * E);
+            for (int i = 0; i < NV; ++i) {
+                const int k = h + (i * NT + u) * E;
+                x[i].load(z + (i < NV / 2 ? k : min(k, nvec ? h + shift - E : 0)));
+            }
         }
     }
-    const float x1 = single ? D::up(z[t0 + u]) : -INFINITY;
+    const float x1 = single ? D::up(z[at1]) : -INFINITY;
 
     // ------------------------------------------------------------ entries
     // of the first wave: p, log2 p and the z they name; in LDS p, z, the id and the owner's list
@@ -232,9 +241,10 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
                 s_p[gi][j] = p[i];
                 s_x[gi][j] = xe[i];
                 s_id[gi][j] = id[i];
-                const int v = id[i] / E;
-                if (real && (id[i] >= t0 || (v >= v0 && v < v1)))
-                    s_next[gi][j] = atomicExch(&s_head[gi][id[i] >= t0 ? id[i] - t0 : (v - v0) % NT], j);
+                const int e = id[i] - h, v = e / E;
+                const bool lone = e < 0 || e >= shift;
+                if (real && (lone ? singles != 0 : v >= v0 && v < v1))
+                    s_next[gi][j] = atomicExch(&s_head[gi][!lone ? (v - v0) % NT : e < 0 ? id[i] : id[i] - shift], j);
             }
         }
         tot = wave_sum(tot);
@@ -274,7 +284,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
                 V y[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (v + i * NT < v1) y[i].load(z + (v + i * NT) * E);
+                    if (v + i * NT < v1) y[i].load(z + h + (v + i * NT) * E);
                 float n = m;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -355,14 +365,14 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
                     x[i].grad(m, c, l2, f);
                 else
                     x[i] = V{};
-                if (i < NV / 2 || i * NT + u < nvec) x[i].store(dz + (i * NT + u) * E);
+                if (i < NV / 2 || i * NT + u < nvec) x[i].store(dz + h + (i * NT + u) * E);
             }
         } else {
             for (int v = v0 + u; v < v1; v += 4 * NT) {
                 V y[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (v + i * NT < v1) y[i].load(z + (v + i * NT) * E);
+                    if (v + i * NT < v1) y[i].load(z + h + (v + i * NT) * E);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (v + i * NT < v1) {
@@ -370,11 +380,11 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
                             y[i].grad(m, c, l2, f);
                         else
                             y[i] = V{};
-                        y[i].store(dz + (v + i * NT) * E);
+                        y[i].store(dz + h + (v + i * NT) * E);
                     }
             }
         }
-        if (single) dz[t0 + u] = D::down(any ? f * ex2(fmaf(x1 - m, c, -l2)) : 0.0f);
+        if (single) dz[at1] = D::down(any ? f * ex2(fmaf(x1 - m, c, -l2)) : 0.0f);
         if (!any || tot != tot) return;
         // this thread's entries: of several with one id the first adds up all, in their order
         for (int j = s_head[gi][u]; j >= 0; j = s_next[gi][j]) {

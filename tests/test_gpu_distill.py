@@ -248,6 +248,30 @@ def test_strides_shapes_and_in_place(dtype):
     assert dz.data_ptr() == place.data_ptr() and torch.equal(loss, want) and torch.equal(place, dwant)
 
 
+# (outputs of one vector or two more than a group's registers hold half of, in 16 bits and in 32)
+@pytest.mark.parametrize("rows,vocab", [(3, 1), (3, 8), (3, 15), (5, 520), (5, 1032), (4100, 2056), (3, 4104), (200, 8200),
+                                        (200, 16392), (195, 32776), (193, 65544), (5, 8200), (3, 16385), (7, 65544)])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_rows_at_any_alignment(rows, vocab, dtype):
+    from lira_amd import distill_topk_loss, distill_topk_loss_and_grad
+    z, ti, tv, w = make(rows, vocab, min(vocab, 7), dtype, seed=vocab)
+    ti[:, 0] = 0
+    ti[1:, -1] = vocab - 1
+    loss, grad, tl, tg = ref(z, ti, tv, 2.0)
+    for off, goff in ((1, 1), (3, 3), (7, 0), (0, 5)):
+        zs = torch.cat([z.new_zeros(off), z.flatten()])[off:].view(rows, vocab)
+        room = torch.full((goff + rows * vocab + 9,), 77.0, device="cuda", dtype=DT[dtype])
+        got, dz = distill_topk_loss_and_grad(zs, ti, tv, 2.0, row_weight=w, grad_out=room[goff:goff + rows * vocab].view(rows, vocab))
+        check_loss(got, loss, tl)
+        check_grad(dz, grad * w.double()[:, None], tg * w.double().abs()[:, None] * 1.001)
+        assert bool((room[:goff] == 77).all()) and bool((room[goff + rows * vocab:] == 77).all())
+    zs.requires_grad_(True)
+    got = distill_topk_loss(zs, ti, tv, 2.0, reduction="none")
+    check_loss(got, loss, tl)
+    (dz,) = torch.autograd.grad(got, zs, w)
+    check_grad(dz, grad * w.double()[:, None], tg * w.double().abs()[:, None] * 1.001)
+
+
 @pytest.mark.parametrize("rows,vocab", [(2, 131072), (300, 4000), (4096, 64)])
 def test_repeats_bit_for_bit_on_streams_and_in_graphs(rows, vocab):
     from lira_amd import distill_topk_loss_and_grad
