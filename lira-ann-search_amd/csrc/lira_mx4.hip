@@ -624,9 +624,14 @@ static int launch_rows(const Product &p, const Rows &r, hipStream_t st) {
     LIRA_HIP_TRY(hipGetLastError());
     return LIRA_OK;
 }
-// Rows that the product packs by itself: so few that every workgroup may do it again.
-static constexpr int64_t kFusedMax = 4;
-static bool fused_rows(int64_t m, int64_t k) { return m <= kFusedMax && m * (planes_of(k) * 68 + 16) <= 49152; }
+// Rows that the product packs by itself: so few that every workgroup may do it again.  Up to 4 always (while they fit
+// LDS); up to 16 of fewer planes, where that costs less than a launch of its own (kernels alone, us, packed here and
+// by themselves: 16 x 8192 x 2048 6.9 and 7.1, 8 x 8192 x 4096 7.2 and 7.5, 16 x 8192 x 4096 10.3 and 7.4; 12 x 40000 x
+// 2048 19.3 and 21.1, 8 x 40000 x 4096 27.3 and 24.5).
+static bool fused_rows(int64_t m, int64_t n, int64_t k) {
+    const int64_t planes = planes_of(k);
+    return (m <= 4 && m * (planes * 68 + 16) <= 49152) || (m <= 16 && m * planes <= (n <= 8192 ? 256 : 192));
+}
 
 // 4096 tiles of 16 columns are enough loads in flight without the planes split (one row, us split and not: 32768 x
 // 4096 18 and 26, 65536 x 4096 32 and 25, 200000 x 900 54 and 19).
@@ -649,6 +654,40 @@ static int linear_rows(const Product &p, const Rows &r, int out_dtype, hipStream
     if (out_dtype == LIRA_DTYPE_BF16) return linear_rows<X, BF16>(p, r, st);
     return linear_rows<X, F16>(p, r, st);
 }
+// The tile of more than 16 rows: the one with the least estimated time.  A launch takes
+// start + planes * plane + load * (tile + planes * step) us, where load is the tiles of a compute unit, between the
+// average and the busiest's; the four numbers of each tile are least squares over 756 products (20 to 4096 rows, 256
+// to 300000 columns, k 128 to 8192, 16-bit results).  On those, the choice is 1.7 % slower than the best tile, in
+// the mean; the largest tile that leaves no compute unit idle was 16 %.  The first three tiles have four sets of
+// waves and take four planes a barrier: less of a step is left bare, so they win while a compute unit has one tile
+// of many planes (37 x 11111 x 5000: 11.8 us by the third, 13.3 by the fifth); the others are small enough in LDS for
+// two or more a unit (37 x 300000 x 128: 11 us by the sixth, 28 by the third).
+static const struct {
+    int tn, tm;
+    float start, plane, tile, step;
+} kTiles[] = {
+    {32, 32, 3.136f, 0.043f, 0.875f, 0.065f},
+    {64, 32, 3.796f, 0.017f, 1.108f, 0.138f},
+    {64, 64, 3.794f, 0.033f, 1.852f, 0.170f},
+    {64, 32, 2.975f, 0.133f, 0.417f, 0.073f},
+    {64, 64, 3.127f, 0.149f, 0.473f, 0.096f},
+    {128, 64, 3.607f, 0.179f, 0.699f, 0.160f},
+    {128, 128, 3.989f, 0.215f, 1.542f, 0.246f},
+    {256, 256, 3.441f, 0.340f, 6.660f, 0.784f},
+};
+static int tile_for(const Product &p) {
+    int best = 0;
+    float least = INFINITY;
+    for (int i = 0; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
+        const auto &t = kTiles[i];
+        const int64_t tiles = ((p.n + t.tn - 1) / t.tn) * ((p.m + t.tm - 1) / t.tm);
+        const float load = 0.5f * ((float)((tiles + 255) / 256) + (float)tiles / 256.0f);
+        const float us = t.start + p.planes * t.plane + load * (t.tile + p.planes * t.step);
+        if (us < least) least = us, best = i;
+    }
+    return best;
+}
+
 template <class D>
 static int product(const Product &p, hipStream_t st) {
     if (p.m <= 16) {
@@ -656,17 +695,16 @@ static int product(const Product &p, hipStream_t st) {
         if (split_planes(p)) return launch_rows<F32, D, 1, 8, false, false>(p, r, st);
         return launch_rows<F32, D, 2, 1, false, false>(p, r, st);
     }
-    // Rows alone decide while one tile takes them all; then the largest tile that still gives each of
-    // the 256 compute units one (k = n = 8192, us a call with the packing of the rows: 64 rows
-    // 16.4 here, 21 on the 64 x 64 tile; 1024 rows 58 on the 128 x 128 tile, 512 tiles of it).
-    const int64_t big = ((p.n + 255) / 256) * ((p.m + 255) / 256), mid = ((p.n + 127) / 128) * ((p.m + 127) / 128);
-    if (p.m <= 32) return launch_tile<32, 32, 2, 2, 2, 4, 4, D>(p, st);
-    if (p.m <= 64) return launch_tile<32, 64, 2, 2, 2, 3, 4, D>(p, st);
-    if (big >= 256) return launch_tile<256, 256, 2, 4, 1, 4, 1, D>(p, st);
-    if (mid >= 256) return launch_tile<128, 128, 2, 2, 1, 4, 1, D>(p, st);
-    // (one tile a compute unit: all of its LDS, twice the planes a barrier: 128 rows 18.5 us, else 22)
-    if (((p.n + 63) / 64) * ((p.m + 63) / 64) <= 256) return launch_tile<64, 64, 2, 2, 2, 4, 4, D>(p, st);
-    return launch_tile<64, 64, 2, 2, 2, 4, 2, D>(p, st);
+    switch (tile_for(p)) {
+    case 0: return launch_tile<32, 32, 1, 2, 4, 4, 4, D>(p, st);
+    case 1: return launch_tile<64, 32, 2, 1, 4, 4, 4, D>(p, st);
+    case 2: return launch_tile<64, 64, 2, 1, 4, 4, 4, D>(p, st);
+    case 3: return launch_tile<64, 32, 2, 2, 1, 4, 1, D>(p, st);
+    case 4: return launch_tile<64, 64, 2, 2, 1, 4, 1, D>(p, st);
+    case 5: return launch_tile<128, 64, 2, 2, 1, 4, 1, D>(p, st);
+    case 6: return launch_tile<128, 128, 2, 2, 1, 4, 1, D>(p, st);
+    default: return launch_tile<256, 256, 2, 4, 1, 4, 1, D>(p, st);
+    }
 }
 static int product(const Product &p, int out_dtype, hipStream_t st) {
     if (out_dtype == LIRA_DTYPE_F32) return product<F32>(p, st);
@@ -733,7 +771,7 @@ int lira_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, int64_t a_p
 int lira_mx4_linear_workspace_size(int64_t m, int64_t n, int64_t k, size_t *bytes) {
     if (!bytes) return fail(LIRA_EINVAL, "NULL buffer");
     if (m < 0 || n < 0 || k <= 0) return fail(LIRA_EINVAL, "bad shape");
-    *bytes = m == 0 || n == 0 || fused_rows(m, k) ? 0 : (size_t)(planes_of(k) * m * 68);
+    *bytes = m == 0 || n == 0 || fused_rows(m, n, k) ? 0 : (size_t)(planes_of(k) * m * 68);
     return LIRA_OK;
 }
 

@@ -189,6 +189,26 @@ def test_linear(m, n, k, dtype):
         check_product(mx4_matmul(mx4_quantize(x), w, b, act, alpha, out_dtype=dt), xv, wv, alpha, bv, act, dt)
 
 
+# (one of every tile, in the order of the kernels' list; then rows that the product packs by itself, and that it no longer does)
+@pytest.mark.parametrize("m,n,k", [(17, 700, 2000), (20, 9000, 4000), (50, 9001, 4000), (20, 20001, 300), (60, 20001, 300),
+                                   (130, 20001, 40), (65, 65537, 2000), (700, 20001, 1000), (16, 1000, 2048), (5, 8200, 4096),
+                                   (12, 40000, 2000), (13, 70001, 900), (16, 9000, 1700), (9, 300, 3600), (6, 501, 5000)])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_linear_by_every_tile(m, n, k, dtype):
+    from lira_amd import mx4_linear, mx4_matmul, mx4_quantize
+    g = gen(m + n + k)
+    x = torch.randn(m, k, generator=g, device="cuda").to(DT[dtype])
+    w = mx4_quantize(torch.randn(n, k, generator=g, device="cuda") * k ** -0.5)
+    bias = torch.randn(n, generator=g, device="cuda")
+    xv, wt = mx4_quantize(x).dequantize().double(), w.dequantize().double().t().contiguous()
+    want, mag = 0.5 * (xv @ wt) + bias, 0.5 * (xv.abs() @ wt.abs()) + bias.abs()
+    tol = (k / 32 + 4) * 2.0 ** -22 * mag  # (as in check_product)
+    tol = tol + torch.finfo(DT[dtype]).eps / 2 * (want.abs() + tol) + torch.finfo(DT[dtype]).tiny
+    for got in (mx4_linear(x, w, bias, alpha=0.5), mx4_matmul(mx4_quantize(x), w, bias, alpha=0.5, out_dtype=DT[dtype])):
+        err = (got.double() - want).abs()
+        assert bool((err <= tol).all()), float((err / tol).max())
+
+
 @pytest.mark.parametrize("m,n", [(0, 40), (40, 0), (0, 0)])
 def test_linear_of_nothing(m, n):
     from lira_amd import mx4_linear, mx4_quantize
