@@ -2,6 +2,7 @@
 // cores (layout and format: lira_mx4.hpp).
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "lira_internal.hpp"
 #include "lira_mx4.hpp"
@@ -190,18 +191,21 @@ __device__ __forceinline__ f32x4 mfma(i32x4 b, int sb, i32x4 a, int sa, f32x4 ac
 // waves split the tile; where a tile is small, WK such sets of waves split a slot's planes (there
 // is one barrier a slot, and a set's LDS reads and matrix instructions wait for each
 // other: with more sets, less of that is left bare) and join their sums in LDS in a fixed order.
-template <int TN, int TM, int WN, int WM, int WK, int SLOTS, int PS>
+// PACK: the rows come as they are and are packed into their places by the workgroup itself, all planes (no more than
+// there are slots) before the first product: a launch and the packed rows' way through memory less.
+template <int TN, int TM, int WN, int WM, int WK, int SLOTS, int PS, bool PACK = false>
 struct Tile {
     static constexpr int NW = WN * WM * WK, FN = TN / WN / 16, FM = TM / WM / 16;
-    static constexpr int kCodeJobs = (TN + TM) / 16;                               // of 16 rows, a plane
-    static constexpr int kNb = (TN + 63) / 64, kScaleJobs = kNb + (TM + 63) / 64;  // of up to 64 rows, a plane
+    static constexpr int kNb = (TN + 63) / 64, kNa = (TM + 63) / 64;
+    static constexpr int kCodeJobs = (TN + (PACK ? 0 : TM)) / 16;  // of 16 rows, a plane
+    static constexpr int kScaleJobs = kNb + (PACK ? 0 : kNa);      // of up to 64 rows, a plane
     // per wave and slot (every wave makes the same number, so that it can wait by count: one without
     // a job of its own repeats another's)
     static constexpr int kCodeLoads = (kCodeJobs * PS + NW - 1) / NW, kScaleLoads = (kScaleJobs * PS + NW - 1) / NW;
     static constexpr int kLoads = kCodeLoads + kScaleLoads;
     // a plane of a slot: the codes of both sides, then their scales, 256 bytes a job (a side under 64 rows
     // fills its job's lanes by repeating its last row)
-    static constexpr int kScaleAt = (TN + TM) * 64, kPlaneBytes = kScaleAt + kScaleJobs * 256;
+    static constexpr int kScaleAt = (TN + TM) * 64, kPlaneBytes = kScaleAt + (kNb + kNa) * 256;
     static constexpr int kBytes = SLOTS * PS * kPlaneBytes;
     // LDS that the sets' sums, or the rows on their way out (16 a wave, 16 bytes apart), take in the slots' place
     template <class D>
@@ -209,6 +213,7 @@ struct Tile {
         return WK > 1 ? NW * FN * FM * 1024 : NW * 16 * (TN / WN * (int)sizeof(typename D::T) + 16);
     }
     static_assert(PS % WK == 0, "the sets split a slot's planes evenly");
+    static_assert(!PACK || (PS == 1 && WK == 1), "packed rows: slot s is plane s");
 
     struct Frags {
         i32x4 b[FN], a[FM];
@@ -216,9 +221,16 @@ struct Tile {
     };
 };
 
-template <int TN, int TM, int WN, int WM, int WK, int SLOTS, int PS, class D>
-__global__ __launch_bounds__(WN *WM *WK * 64) void k_mx4_tile(Product P, int tiles_n, int tiles_m) {
-    typedef Tile<TN, TM, WN, WM, WK, SLOTS, PS> C;
+struct Rows {
+    const void *x;  // (m, k), row stride ldx
+    int64_t k, ldx;
+    bool vec;  // first element and row stride are multiples of 16 bytes
+};
+// X: void, or the type of the rows that the tile packs
+template <int TN, int TM, int WN, int WM, int WK, int SLOTS, int PS, class D, class X = void>
+__global__ __launch_bounds__(WN *WM *WK * 64) void k_mx4_tile(Product P, Rows R, int tiles_n, int tiles_m) {
+    constexpr bool PACK = !std::is_void<X>::value;
+    typedef Tile<TN, TM, WN, WM, WK, SLOTS, PS, PACK> C;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -316,6 +328,40 @@ __global__ __launch_bounds__(WN *WM *WK * 64) void k_mx4_tile(Product P, int til
         if (s + kAhead < steps) fetch(s + kAhead);
     };
     for (int s = 0; s < kAhead && s < steps; ++s) fetch(s);
+    if constexpr (PACK) {
+        // 8 elements a thread at a time, as in k_mx4_rows, a plane's all loaded before the first is packed;
+        // the first wait's barrier is behind the last
+        constexpr int U = TM * 16 / (C::NW * 64);
+        const bool whole = R.vec && R.k % 8 == 0;  // (then a run is all in the row or all behind it, and k >= 8)
+        for (int p = 0; p < planes; ++p) {
+            const int run = threadIdx.x & 15, block = run >> 2;
+            const int64_t at = p * kPlane + run * 8;
+            uint8_t *slot = smem + p * C::kPlaneBytes;
+            float v[U][8];
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const uint32_t row = i * (C::NW * 4) + (threadIdx.x >> 4);
+                const typename X::T *x = (const typename X::T *)R.x + (m0 + min(row, mlast)) * R.ldx;
+                if (whole)
+                    load_run<X, true, 8>(x, min(at, R.k - 8), R.k, v[i]);
+                else
+                    load_run<X, false, 8>(x, at, R.k, v[i]);
+            }
+            if (whole && at >= R.k) {
+#pragma unroll
+                for (int i = 0; i < U; ++i)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                const uint32_t row = i * (C::NW * 4) + (threadIdx.x >> 4), z = scale_code(quad_max(v[i]));
+                *reinterpret_cast<uint32_t *>(slot + (TN + row) * 64 + ((uint32_t)block ^ turn(row)) * 16 + (run & 3) * 4) =
+                    z == 255 ? 0u : to_codes(v[i], scale_operand(z));
+                if ((run & 3) == 0) slot[C::kScaleAt + C::kNb * 256 + row * 4 + block] = (uint8_t)z;
+            }
+        }
+    }
     for (int s = 0; s < steps; ++s) {
         arrive(s);
         typename C::Frags f[PS / WK];
@@ -403,10 +449,6 @@ __global__ __launch_bounds__(WN *WM *WK * 64) void k_mx4_tile(Product P, int til
 // few planes or many columns: four waves, each of its own columns, that go on to the next ones without a gap.  FUSED: the rows of x are
 // packed here, 32 elements a thread, while the first planes of W are on their way; else they come
 // packed and are read from the cache.
-struct Rows {
-    const void *x;  // FUSED: (m, k), row stride ldx
-    int64_t k, ldx;
-};
 template <class X, class D, int NB, int KS, bool FUSED, bool VEC>
 __global__ __launch_bounds__(KS == 1 ? 256 : KS * 64, 4) void k_mx4_rows(Product P, Rows R) {
     constexpr int U = KS == 1 ? 2 : FUSED ? 3 : 4;  // planes in flight
@@ -591,12 +633,12 @@ static int dequantize(const uint8_t *codes, const uint8_t *scales, int64_t plane
     return LIRA_OK;
 }
 
-template <int TN, int TM, int WN, int WM, int WK, int SLOTS, int PS, class D>
-static int launch_tile(const Product &p, hipStream_t st) {
-    typedef Tile<TN, TM, WN, WM, WK, SLOTS, PS> C;
+template <int TN, int TM, int WN, int WM, int WK, int SLOTS, int PS, class D, class X = void>
+static int launch_tile(const Product &p, hipStream_t st, const Rows &r = {nullptr, 0, 0, false}) {
+    typedef Tile<TN, TM, WN, WM, WK, SLOTS, PS, !std::is_void<X>::value> C;
     static_assert(C::kBytes <= 163840 && C::template epilogue_bytes<D>() <= C::kBytes, "160 KB of LDS");
     static std::atomic<uint64_t> latch{0};
-    const void *fn = (const void *)&k_mx4_tile<TN, TM, WN, WM, WK, SLOTS, PS, D>;
+    const void *fn = (const void *)&k_mx4_tile<TN, TM, WN, WM, WK, SLOTS, PS, D, X>;
     LIRA_HIP_TRY(set_smem_attr_once(latch, fn, C::kBytes));
     // (few planes: only the slots that they fill, so that more workgroups share a compute unit:
     // 10000 x 1024 x 128 20 us -> 14)
@@ -604,8 +646,8 @@ static int launch_tile(const Product &p, hipStream_t st) {
     const int bytes = std::min<int>(C::kBytes, std::max<int>(slots, C::template epilogue_bytes<D>()));
     const int64_t tn = (p.n + TN - 1) / TN, tm = (p.m + TM - 1) / TM;
     if (tn * tm > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "product: too many tiles for one launch");
-    hipLaunchKernelGGL((k_mx4_tile<TN, TM, WN, WM, WK, SLOTS, PS, D>), dim3((unsigned)(tn * tm)), dim3(C::NW * 64), bytes, st, p,
-                       (int)tn, (int)tm);
+    hipLaunchKernelGGL((k_mx4_tile<TN, TM, WN, WM, WK, SLOTS, PS, D, X>), dim3((unsigned)(tn * tm)), dim3(C::NW * 64), bytes, st, p,
+                       r, (int)tn, (int)tm);
     LIRA_HIP_TRY(hipGetLastError());
     return LIRA_OK;
 }
@@ -628,7 +670,7 @@ static int launch_rows(const Product &p, const Rows &r, hipStream_t st) {
 // LDS); up to 16 of fewer planes, where that costs less than a launch of its own (kernels alone, us, packed here and
 // by themselves: 16 x 8192 x 2048 6.9 and 7.1, 8 x 8192 x 4096 7.2 and 7.5, 16 x 8192 x 4096 10.3 and 7.4; 12 x 40000 x
 // 2048 19.3 and 21.1, 8 x 40000 x 4096 27.3 and 24.5).
-static bool fused_rows(int64_t m, int64_t n, int64_t k) {
+static bool rows_packed(int64_t m, int64_t n, int64_t k) {
     const int64_t planes = planes_of(k);
     return (m <= 4 && m * (planes * 68 + 16) <= 49152) || (m <= 16 && m * planes <= (n <= 8192 ? 256 : 192));
 }
@@ -639,20 +681,13 @@ static bool split_planes(const Product &p) { return p.planes >= 8 && (p.n + 15) 
 
 template <class X, class D>
 static int linear_rows(const Product &p, const Rows &r, hipStream_t st) {
-    const bool vec = ((uintptr_t)r.x & 15) == 0 && (r.ldx * sizeof(typename X::T)) % 16 == 0;
     // (32 columns a workgroup where that still leaves each compute unit one: the rows are packed half as often; 4 x 8192
     // x 8192 12.4 us, 14.4 with 16)
     if (split_planes(p) && p.n >= 256 * 32)
-        return vec ? launch_rows<X, D, 2, 8, true, true>(p, r, st) : launch_rows<X, D, 2, 8, true, false>(p, r, st);
+        return r.vec ? launch_rows<X, D, 2, 8, true, true>(p, r, st) : launch_rows<X, D, 2, 8, true, false>(p, r, st);
     if (split_planes(p))
-        return vec ? launch_rows<X, D, 1, 8, true, true>(p, r, st) : launch_rows<X, D, 1, 8, true, false>(p, r, st);
-    return vec ? launch_rows<X, D, 2, 1, true, true>(p, r, st) : launch_rows<X, D, 2, 1, true, false>(p, r, st);
-}
-template <class X>
-static int linear_rows(const Product &p, const Rows &r, int out_dtype, hipStream_t st) {
-    if (out_dtype == LIRA_DTYPE_F32) return linear_rows<X, F32>(p, r, st);
-    if (out_dtype == LIRA_DTYPE_BF16) return linear_rows<X, BF16>(p, r, st);
-    return linear_rows<X, F16>(p, r, st);
+        return r.vec ? launch_rows<X, D, 1, 8, true, true>(p, r, st) : launch_rows<X, D, 1, 8, true, false>(p, r, st);
+    return r.vec ? launch_rows<X, D, 2, 1, true, true>(p, r, st) : launch_rows<X, D, 2, 1, true, false>(p, r, st);
 }
 // The tile of more than 16 rows: the one with the least estimated time.  A launch takes
 // start + planes * plane + load * (tile + planes * step) us, where load is the tiles of a compute unit, between the
@@ -691,7 +726,7 @@ static int tile_for(const Product &p) {
 template <class D>
 static int product(const Product &p, hipStream_t st) {
     if (p.m <= 16) {
-        const Rows r = {nullptr, 0, 0};
+        const Rows r = {nullptr, 0, 0, false};
         if (split_planes(p)) return launch_rows<F32, D, 1, 8, false, false>(p, r, st);
         return launch_rows<F32, D, 2, 1, false, false>(p, r, st);
     }
@@ -705,6 +740,26 @@ static int product(const Product &p, hipStream_t st) {
     case 6: return launch_tile<128, 128, 2, 2, 1, 4, 1, D>(p, st);
     default: return launch_tile<256, 256, 2, 4, 1, 4, 1, D>(p, st);
     }
+}
+// More rows, packed by their tiles: of whole runs of 8, and so few planes and tiles a compute unit that this takes no
+// longer than a launch of its own does (kernels alone, fp32, us, packed here and by themselves: 1000 x 256 x 128 5.2
+// and 5.2, 4000 x 1024 x 128 6.8 and 8.0, 50000 x 256 x 128 14.8 and 19.2, 1000 x 1024 x 256 6.5 and 6.1; 1000 x 1024 x
+// 384 9.3 and 6.4; a call from Python takes 4 less).  Rows that are not aligned take 7.6 and 11.4, not 5.2 and 6.8.
+static bool tile_packed(int64_t m, int64_t n, int64_t k) {
+    const int64_t planes = planes_of(k), load = (((n + 127) / 128) * ((m + 63) / 64) + 255) / 256;
+    return m > 16 && k % 8 == 0 && planes <= 2 && load * planes <= 10;
+}
+static bool packed_inside(int64_t m, int64_t n, int64_t k) { return rows_packed(m, n, k) || tile_packed(m, n, k); }
+template <class X, class D>
+static int linear(const Product &p, const Rows &r, hipStream_t st) {
+    if (p.m <= 16) return linear_rows<X, D>(p, r, st);
+    return launch_tile<128, 64, 2, 2, 1, 4, 1, D, X>(p, st, r);
+}
+template <class X>
+static int linear(const Product &p, const Rows &r, int out_dtype, hipStream_t st) {
+    if (out_dtype == LIRA_DTYPE_F32) return linear<X, F32>(p, r, st);
+    if (out_dtype == LIRA_DTYPE_BF16) return linear<X, BF16>(p, r, st);
+    return linear<X, F16>(p, r, st);
 }
 static int product(const Product &p, int out_dtype, hipStream_t st) {
     if (out_dtype == LIRA_DTYPE_F32) return product<F32>(p, st);
@@ -771,7 +826,7 @@ int lira_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, int64_t a_p
 int lira_mx4_linear_workspace_size(int64_t m, int64_t n, int64_t k, size_t *bytes) {
     if (!bytes) return fail(LIRA_EINVAL, "NULL buffer");
     if (m < 0 || n < 0 || k <= 0) return fail(LIRA_EINVAL, "bad shape");
-    *bytes = m == 0 || n == 0 || fused_rows(m, n, k) ? 0 : (size_t)(planes_of(k) * m * 68);
+    *bytes = m == 0 || n == 0 || packed_inside(m, n, k) ? 0 : (size_t)(planes_of(k) * m * 68);
     return LIRA_OK;
 }
 
@@ -792,10 +847,10 @@ int lira_mx4_linear(const void *x, int dtype, int64_t m, int64_t k, int64_t ldx,
     if (!need) {
         const Product p = {nullptr, nullptr, b_codes, b_scales, 0, b_plane_rows, m, n, ldo,
                            (int)planes_of(k), epilogue(bias, alpha, act, n), out};
-        const Rows r = {x, k, ldx};
-        if (dtype == LIRA_DTYPE_F32) return linear_rows<F32>(p, r, out_dtype, (hipStream_t)stream);
-        if (dtype == LIRA_DTYPE_BF16) return linear_rows<BF16>(p, r, out_dtype, (hipStream_t)stream);
-        return linear_rows<F16>(p, r, out_dtype, (hipStream_t)stream);
+        const Rows r = {x, k, ldx, ((uintptr_t)x & 15) == 0 && (ldx * (dtype == LIRA_DTYPE_F32 ? 4 : 2)) % 16 == 0};
+        if (dtype == LIRA_DTYPE_F32) return linear<F32>(p, r, out_dtype, (hipStream_t)stream);
+        if (dtype == LIRA_DTYPE_BF16) return linear<BF16>(p, r, out_dtype, (hipStream_t)stream);
+        return linear<F16>(p, r, out_dtype, (hipStream_t)stream);
     }
     uint8_t *ac = (uint8_t *)workspace, *as = ac + planes_of(k) * m * 64;
     if (int rc = lira_mx4_quantize(x, dtype, m, k, ldx, ac, as, m, stream)) return rc;

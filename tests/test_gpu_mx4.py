@@ -209,6 +209,30 @@ def test_linear_by_every_tile(m, n, k, dtype):
         assert bool((err <= tol).all()), float((err / tol).max())
 
 
+# (rows packed by the product itself or by a launch of their own: the same numbers in the same order, so the same bits)
+@pytest.mark.parametrize("m,n,k", [(17, 1, 8), (17, 130, 16), (64, 257, 128), (65, 129, 96), (1000, 333, 104), (300, 200, 256), (129, 1000, 248),
+                                   (40, 9001, 136), (4000, 64, 200), (20, 100001, 64), (64, 64, 8), (16, 70, 2000), (10, 40000, 2000)])
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("dtype", list(DT))
+def test_rows_packed_inside(m, n, k, offset, dtype):
+    from lira_amd import mx4_linear, mx4_matmul, mx4_quantize
+    g = gen(m + n + k)
+    room = torch.full((m, k + 11 * offset), float("nan"), device="cuda", dtype=DT[dtype])
+    x = room[:, offset:offset + k]
+    x.copy_(torch.randn(m, k, generator=g, device="cuda") * torch.exp(4 * torch.randn(m, 1, generator=g, device="cuda")))
+    if m > 20:
+        x[3, k // 2] = float("inf")
+        x[5] = 0
+    w = mx4_quantize(torch.randn(n, k, generator=g, device="cuda"))
+    out = torch.full((m + 1, n + 3), 7.0, device="cuda", dtype=DT[dtype])
+    mx4_linear(x, w, out=out[:m, :n])
+    want = mx4_matmul(mx4_quantize(x), w, out_dtype=DT[dtype])
+    assert torch.equal(out[:m, :n].nan_to_num(nan=-1.0), want.nan_to_num(nan=-1.0))
+    assert bool((out[m] == 7).all()) and bool((out[:, n:] == 7).all())
+    if m > 20:
+        assert bool(out[3, :n].isnan().all()) and not bool(out[5, :n].any())
+
+
 @pytest.mark.parametrize("m,n", [(0, 40), (40, 0), (0, 0)])
 def test_linear_of_nothing(m, n):
     from lira_amd import mx4_linear, mx4_quantize
