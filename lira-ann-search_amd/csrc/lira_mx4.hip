@@ -741,13 +741,14 @@ static int product(const Product &p, hipStream_t st) {
     default: return launch_tile<256, 256, 2, 4, 1, 4, 1, D>(p, st);
     }
 }
-// More rows, packed by their tiles: of whole runs of 8, and so few planes and tiles a compute unit that this takes no
-// longer than a launch of its own does (kernels alone, fp32, us, packed here and by themselves: 1000 x 256 x 128 5.2
-// and 5.2, 4000 x 1024 x 128 6.8 and 8.0, 50000 x 256 x 128 14.8 and 19.2, 1000 x 1024 x 256 6.5 and 6.1; 1000 x 1024 x
-// 384 9.3 and 6.4; a call from Python takes 4 less).  Rows that are not aligned take 7.6 and 11.4, not 5.2 and 6.8.
+// More rows, packed by their tiles: of whole runs of 8, for half a tile's columns or more, and of so few planes and
+// tiles a compute unit that this takes no longer than a launch of its own does (kernels alone, fp32, us, packed here
+// and by themselves: 1000 x 256 x 128 5.2 and 5.2, 4000 x 1024 x 128 6.8 and 8.0, 50000 x 256 x 128 14.8 and 19.2,
+// 1000 x 1024 x 256 6.5 and 6.1; 1000 x 1024 x 384 9.3 and 6.4; a call from Python takes 4 less).  Rows that are not
+// aligned take 7.6 and 11.4, not 5.2 and 6.8.
 static bool tile_packed(int64_t m, int64_t n, int64_t k) {
     const int64_t planes = planes_of(k), load = (((n + 127) / 128) * ((m + 63) / 64) + 255) / 256;
-    return m > 16 && k % 8 == 0 && planes <= 2 && load * planes <= 10;
+    return m > 16 && n >= 64 && k % 8 == 0 && planes <= 2 && load * planes <= 10;
 }
 static bool packed_inside(int64_t m, int64_t n, int64_t k) { return rows_packed(m, n, k) || tile_packed(m, n, k); }
 template <class X, class D>

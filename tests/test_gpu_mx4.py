@@ -210,7 +210,7 @@ def test_linear_by_every_tile(m, n, k, dtype):
 
 
 # (rows packed by the product itself or by a launch of their own: the same numbers in the same order, so the same bits)
-@pytest.mark.parametrize("m,n,k", [(17, 1, 8), (17, 130, 16), (64, 257, 128), (65, 129, 96), (1000, 333, 104), (300, 200, 256), (129, 1000, 248),
+@pytest.mark.parametrize("m,n,k", [(17, 64, 8), (17, 1, 8), (17, 130, 16), (64, 257, 128), (65, 129, 96), (1000, 333, 104), (300, 200, 256), (129, 1000, 248),
                                    (40, 9001, 136), (4000, 64, 200), (20, 100001, 64), (64, 64, 8), (16, 70, 2000), (10, 40000, 2000)])
 @pytest.mark.parametrize("offset", [0, 1])
 @pytest.mark.parametrize("dtype", list(DT))
