@@ -106,32 +106,35 @@ class _Loss(torch.autograd.Function):
         stats = torch.empty((head[2], 4), dtype=torch.float32, device=dev)
         loss = _forward(head, dev, stats, None, None)
         ctx.save_for_backward(z, ids, tv, lse, stats)
-        ctx.t, ctx.factor = t, None
+        ctx.sizes, ctx.factor = (head[1], head[2], head[3], head[4], head[6], head[8], t), None
         if reduction == "none":
             return loss
         out = torch.empty(2, dtype=torch.float32, device=dev)
         _lib.run("lira_distill_reduce", loss.data_ptr(), stats.data_ptr(), head[2], reduction == "mean", out.data_ptr(),
                  raw_stream(dev.index))
-        ctx.factor = out[1]
+        if reduction == "mean":
+            ctx.factor = out[1]  # (of a sum it is 1)
         return out[0].clone()
 
     @staticmethod
     def backward(ctx, g):
         if torch.is_grad_enabled():
             raise RuntimeError("distill_topk_loss has no second derivative (create_graph=True)")
-        z, ids, tv, lse, stats = ctx.saved_tensors  # (not always the tensors of the forward pass: hooks may have moved them)
-        z, dev = _rows(z)[0], z.device
-        head = _head(z, ids, tv, lse, ctx.t)
-        rows, vocab = head[2], head[3]
-        with on(dev):
-            if ctx.factor is not None:
-                g = g * ctx.factor
-            whole = g.dim() == 0 or (rows > 1 and g.stride(0) == 0)  # one factor for all rows
-            if not whole:
-                g = g.contiguous()
-            dz = torch.empty((rows, vocab), dtype=z.dtype, device=dev)
-            _lib.run("lira_distill_topk_backward", *head, stats.data_ptr(), g.data_ptr(), 0 if whole else 1,
-                     dz.data_ptr(), vocab, raw_stream(dev.index))
+        # (not always the tensors of the forward pass: hooks may have moved them.  The engine has made their device and
+        # the forward pass's stream the current ones.)
+        z, ids, tv, lse, stats = ctx.saved_tensors
+        dtype, rows, vocab, ld, bits, top, t = ctx.sizes
+        if z.stride() != (ld, 1):
+            z, ld = _rows(z)
+        if ctx.factor is not None:
+            g = g * ctx.factor
+        whole = g.dim() == 0 or (rows > 1 and g.stride(0) == 0)  # one factor for all rows
+        if not whole:
+            g = g.contiguous()
+        dz = torch.empty((rows, vocab), dtype=z.dtype, device=z.device)
+        _lib.run("lira_distill_topk_backward", z.data_ptr(), dtype, rows, vocab, ld, ids.data_ptr(), bits, tv.data_ptr(), top, t,
+                 None if lse is None else lse.data_ptr(), stats.data_ptr(), g.data_ptr(), 0 if whole else 1, dz.data_ptr(),
+                 vocab, raw_stream(z.device.index))
         return dz, None, None, None, None, None
 
 
