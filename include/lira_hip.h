@@ -408,8 +408,8 @@ int lira_mx4_linear(const void *x, int dtype, int64_t m, int64_t k, int64_t ldx,
  *   dz        NULL: the loss alone.  scale_stride 0: row_scale holds one factor
  *             for all rows; row_scale NULL: 1
  * fp32 sums in an order that the shape and the rows' alignment to 16 bytes fix
- * (results do not vary from run to run), dz rounded once.  Device pointers of the current device, stream-ordered, asynchronous,
- * capturable.
+ * (results do not vary from run to run), dz rounded once.  Device pointers of the
+ * current device, stream-ordered, asynchronous, capturable.
  * lira_distill_reduce: out[0] = sum of loss, or (mean) the mean over the rows
  * that count; out[1] = the factor of every row's gradient, 1 or 1 / count.
  */
