@@ -35,6 +35,8 @@ _HERE = contextlib.nullcontext()
 def on(device: torch.device, stream=None):
     """The context a call runs in: the tensors' device, and ``stream`` as the current one, so that
     whatever the call allocates belongs to the stream that uses it."""
+    if device.type != "cuda":
+        raise ValueError(f"the tensors must be on the GPU, not on {device}")
     if stream is not None:
         if stream.device != device:
             raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
@@ -73,15 +75,22 @@ def _no_grad(t) -> None:
 
 class MX4Tensor:
     """Packed rows: ``codes`` (P, n, 64) uint8, ``scales`` (P, n, 4) uint8, P = ceil(k / 128)
-    planes of 128 elements (include/lira_hip.h).  Row ranges ``t[lo:hi]`` are views."""
+    planes of 128 elements (include/lira_hip.h).  Row ranges ``t[lo:hi]`` are views.  Copies (``copy``,
+    ``pickle``, ``torch.save``) are of the two tensors and k."""
 
-    # (what mx4_quantize packs is one buffer, whose two views are made when they are asked for)
-    __slots__ = ("_codes", "_scales", "_buf", "k", "n", "plane_rows", "device", "codes_ptr", "scales_ptr")
+    # (what mx4_quantize packs is one buffer, whose two views are made when they are asked for; addresses are
+    # read from the tensors at each call, never kept beside them)
+    __slots__ = ("_codes", "_scales", "_buf", "k", "n", "plane_rows")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int):
-        k = int(k)
         for t, w, name in ((codes, 64, "codes"), (scales, 4, "scales")):
-            if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.uint8 or t.dim() != 3 or t.shape[2] != w:
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                raise ValueError(f"{name} must be a (P, n, {w}) uint8 tensor on the GPU")
+        self._set(codes, scales, int(k))
+
+    def _set(self, codes: torch.Tensor, scales: torch.Tensor, k: int) -> None:
+        for t, w, name in ((codes, 64, "codes"), (scales, 4, "scales")):
+            if t.dtype != torch.uint8 or t.dim() != 3 or t.shape[2] != w:
                 raise ValueError(f"{name} must be a (P, n, {w}) uint8 tensor on the GPU")
         p, n, _ = codes.shape
         if k < 1 or p != (k + 127) // 128:
@@ -94,18 +103,32 @@ class MX4Tensor:
                 scales.clone(memory_format=torch.contiguous_format)
             rows = n
         self._codes, self._scales, self._buf = codes, scales, None
-        self.k, self.n, self.plane_rows, self.device = k, n, rows, codes.device
-        self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
+        self.k, self.n, self.plane_rows = k, n, rows
 
     @classmethod
-    def _of(cls, buf: torch.Tensor, device: torch.device, n: int, k: int) -> "MX4Tensor":
+    def _of(cls, buf: torch.Tensor, n: int, k: int) -> "MX4Tensor":
         """Of one buffer: the codes, then the scales."""
         t = object.__new__(cls)
         t._codes = t._scales = None
-        t._buf, t.k, t.n, t.plane_rows, t.device = buf, k, n, n, device
-        t.codes_ptr = buf.data_ptr()
-        t.scales_ptr = t.codes_ptr + (k + 127) // 128 * n * 64
+        t._buf, t.k, t.n, t.plane_rows = buf, k, n, n
         return t
+
+    def __reduce__(self):
+        return _restored, (self.codes, self.scales, self.k)
+
+    @property
+    def device(self) -> torch.device:
+        return (self._buf if self._codes is None else self._codes).device
+
+    @property
+    def codes_ptr(self) -> int:
+        return (self._buf if self._codes is None else self._codes).data_ptr()
+
+    @property
+    def scales_ptr(self) -> int:
+        if self._scales is None:
+            return self._buf.data_ptr() + (self.k + 127) // 128 * self.n * 64
+        return self._scales.data_ptr()
 
     @property
     def codes(self) -> torch.Tensor:
@@ -145,12 +168,20 @@ class MX4Tensor:
     def __getitem__(self, rows: slice) -> "MX4Tensor":
         if not isinstance(rows, slice) or rows.step not in (None, 1):
             raise TypeError("an MX4Tensor is cut by a range of rows, t[lo:hi]")
-        return MX4Tensor(self.codes[:, rows], self.scales[:, rows], self.k)
+        return _restored(self.codes[:, rows], self.scales[:, rows], self.k)
 
     def dequantize(self, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None,
                    stream=None) -> torch.Tensor:
         """The rows as numbers, (n, k): exact in float32, rounded once to the 16-bit types."""
         return mx4_dequantize(self, dtype, out, stream)
+
+
+def _restored(codes: torch.Tensor, scales: torch.Tensor, k: int) -> MX4Tensor:
+    """What copies, and views of rows, are made by: on whatever device the tensors are (torch.load may have put them
+    into host memory, where no operator takes them)."""
+    t = object.__new__(MX4Tensor)
+    t._set(codes, scales, k)
+    return t
 
 
 def mx4_quantize(x: torch.Tensor, stream=None) -> MX4Tensor:
@@ -164,7 +195,7 @@ def mx4_quantize(x: torch.Tensor, stream=None) -> MX4Tensor:
     dev = x.device
     with on(dev, stream):
         x, ld = _rows(x)
-        t = MX4Tensor._of(torch.empty(p * n * 68, dtype=torch.uint8, device=dev), dev, n, k)
+        t = MX4Tensor._of(torch.empty(p * n * 68, dtype=torch.uint8, device=dev), n, k)
         _lib.run("lira_mx4_quantize", x.data_ptr(), DTYPES[x.dtype], n, k, ld, t.codes_ptr, t.scales_ptr, n,
                  raw_stream(dev.index))
     return t
