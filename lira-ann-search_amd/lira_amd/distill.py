@@ -18,6 +18,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .mx4 import DTYPES, check_rows, on, raw_stream, _rows
@@ -166,7 +167,8 @@ def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_
     """(loss (...), grad (..., vocab)): every row's loss as distill_topk_loss(reduction="none")
     gives it, and the gradient of sum(row_weight * loss) with respect to the logits, for
     ``logits.backward(grad)``.  row_weight (...): None = 1.  grad_out: where the gradient goes, a
-    contiguous tensor like the logits; the logits themselves are allowed."""
+    contiguous tensor like the logits; the logits themselves are allowed (an in-place change to autograd: the
+    backward pass of an operation that saved them, as tanh does, is then refused by torch)."""
     check_device(logits)
     dev = logits.device
     with on(dev, stream):
@@ -179,6 +181,7 @@ def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_
             raise ValueError("grad_out must be a contiguous tensor of the logits' shape, type and device")
         else:
             dz = grad_out
+            increment_version(dz)  # (autograd may have saved it: the logits' own operation, where it is the logits)
         z = _rows(z)[0]  # (perhaps a copy: held until the launch, the head has its address alone)
         loss = _forward(_head(z, ids, tv, lse, temperature), dev, None, w, dz)
     return loss if len(lead) == 1 else loss.view(lead), dz

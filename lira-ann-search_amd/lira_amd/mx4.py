@@ -19,6 +19,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 
@@ -221,6 +222,7 @@ def _out(out, shape, dtype, device, *inputs) -> tuple[torch.Tensor, int]:
         if lo < _span(t)[1] and _span(t)[0] < hi:
             raise ValueError("out must not share memory with an input")
     _no_grad(out)
+    increment_version(out)  # (autograd may have saved it)
     return out, out.stride(0) if shape[0] > 1 else max(1, shape[1])
 
 

@@ -42,3 +42,62 @@ def test_copies_outlive_their_original(how):
     idx._packed().scales.zero_()
     D2, I2 = other.search(q, 5)
     assert torch.equal(D, D2) and torch.equal(I, I2)
+
+
+def student(rows=6, vocab=50, top=4, seed=3):
+    g = gen(seed)
+    y = torch.randn(rows, vocab, generator=g, device="cuda", requires_grad=True)
+    tv, ti = torch.topk(torch.randn(rows, vocab, generator=g, device="cuda"), top, dim=1)
+    return y, ti, tv
+
+
+@pytest.mark.parametrize("f", [torch.tanh, torch.sigmoid, torch.exp])
+@pytest.mark.parametrize("detached", [False, True])
+def test_gradient_over_saved_logits_is_seen_by_autograd(f, detached):
+    """The logits are what f saved for its backward pass: once they are overwritten that pass must not run on them."""
+    from lira_amd import distill_topk_loss_and_grad
+    y, ti, tv = student()
+    z = f(y)
+    was = z._version
+    _, dz = distill_topk_loss_and_grad(z, ti, tv, grad_out=z.detach() if detached else z)
+    assert z._version > was
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward(dz.detach().clone())
+
+
+def test_gradient_over_logits_that_nobody_saved():
+    """A layer saves its inputs, not its outputs: its backward pass runs on the gradient in the logits' place."""
+    from lira_amd import distill_topk_loss_and_grad
+    y, ti, tv = student()
+    w = torch.randn(50, 50, generator=gen(9), device="cuda")
+    z = y @ w
+    _, dz = distill_topk_loss_and_grad(z.detach().clone(), ti, tv)
+    want = torch.autograd.grad(z, y, dz)[0]
+    z = y @ w
+    _, dz = distill_topk_loss_and_grad(z, ti, tv, grad_out=z)
+    assert dz is z
+    assert torch.equal(torch.autograd.grad(z, y, dz.detach())[0], want)
+
+
+def test_outputs_of_products_are_seen_by_autograd():
+    from lira_amd import mx4_linear, mx4_matmul, mx4_quantize
+    x = torch.randn(6, 64, generator=gen(4), device="cuda")
+    w = mx4_quantize(torch.randn(50, 64, generator=gen(5), device="cuda"))
+    calls = [lambda out: mx4_linear(x, w, out=out), lambda out: mx4_matmul(mx4_quantize(x), w, out=out),
+             lambda out: w[:6].dequantize(out=out)]
+    for call, cols in zip(calls, (50, 50, 64)):
+        y = torch.randn(6, cols, generator=gen(6), device="cuda", requires_grad=True)
+        z = torch.tanh(y)
+        call(z.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.sum().backward()
+        out = torch.zeros(8, cols, device="cuda")
+        was = out._version
+        call(out[1:7])  # (a view's base too)
+        assert out._version > was
+        with torch.inference_mode():
+            inside = torch.zeros(6, cols, device="cuda")
+            call(inside)
+        again = inside.clone()
+        call(inside)
+        assert torch.equal(inside, again)
