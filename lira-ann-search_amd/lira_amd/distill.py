@@ -21,7 +21,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from .mx4 import DTYPES, check_rows, on, raw_stream, _rows
+from .mx4 import DTYPES, check_rows, on, raw_stream, refuse_shared, _rows
 
 
 def check_device(logits) -> None:
@@ -167,13 +167,15 @@ def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_
     """(loss (...), grad (..., vocab)): every row's loss as distill_topk_loss(reduction="none")
     gives it, and the gradient of sum(row_weight * loss) with respect to the logits, for
     ``logits.backward(grad)``.  row_weight (...): None = 1.  grad_out: where the gradient goes, a
-    contiguous tensor like the logits; the logits themselves are allowed (an in-place change to autograd: the
-    backward pass of an operation that saved them, as tanh does, is then refused by torch)."""
+    contiguous tensor like the logits, which must not share memory with an input; the logits
+    themselves are allowed (an in-place change to autograd: the backward pass of an operation that
+    saved them, as tanh does, is then refused by torch)."""
     check_device(logits)
     dev = logits.device
     with on(dev, stream):
         z, lead, ids, tv, lse = _entries(logits, top_ids, top_logits, temperature, teacher_lse)
         w = _row_values(row_weight, "row_weight", lead, dev)
+        z = _rows(z)[0]  # (perhaps a copy: held until the launch, the head has its address alone)
         if grad_out is None:
             dz = torch.empty(logits.shape, dtype=z.dtype, device=dev)
         elif not isinstance(grad_out, torch.Tensor) or grad_out.shape != logits.shape or grad_out.dtype != z.dtype \
@@ -181,7 +183,8 @@ def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_
             raise ValueError("grad_out must be a contiguous tensor of the logits' shape, type and device")
         else:
             dz = grad_out
+            same = dz.data_ptr() == z.data_ptr() and z.is_contiguous()  # (the logits' own places)
+            refuse_shared(dz, "grad_out (but for the logits themselves)", None if same else z, ids, tv, lse, w)
             increment_version(dz)  # (autograd may have saved it: the logits' own operation, where it is the logits)
-        z = _rows(z)[0]  # (perhaps a copy: held until the launch, the head has its address alone)
         loss = _forward(_head(z, ids, tv, lse, temperature), dev, None, w, dz)
     return loss if len(lead) == 1 else loss.view(lead), dz

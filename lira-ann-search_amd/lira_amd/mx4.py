@@ -69,6 +69,23 @@ def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     return x, k
 
 
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The addresses from t's first element to past its last one."""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def refuse_shared(out: torch.Tensor, name: str, *inputs) -> None:
+    """An output may not lie over an input (a tensor or None), which other workgroups still read."""
+    lo, hi = _span(out)
+    for t in inputs:
+        if t is not None:
+            a, b = _span(t)
+            if lo < b and a < hi:
+                raise ValueError(f"{name} must not share memory with an input")
+
+
 def _no_grad(t) -> None:
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError("the 4-bit operators have no gradient: call them under torch.no_grad() or on detached tensors")
@@ -202,13 +219,6 @@ def mx4_quantize(x: torch.Tensor, stream=None) -> MX4Tensor:
     return t
 
 
-def _span(t: torch.Tensor) -> tuple[int, int]:
-    """The addresses from t's first element to past its last one."""
-    if t.numel() == 0:
-        return t.data_ptr(), t.data_ptr()
-    return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-
-
 def _out(out, shape, dtype, device, *inputs) -> tuple[torch.Tensor, int]:
     """Where the result goes, and its row stride; not over an input, which other workgroups still read."""
     if out is None:
@@ -217,10 +227,7 @@ def _out(out, shape, dtype, device, *inputs) -> tuple[torch.Tensor, int]:
         raise ValueError(f"out must be a {shape} {dtype} tensor on {device}")
     if shape[1] > 1 and out.stride(1) != 1 or shape[0] > 1 and out.stride(0) < shape[1]:
         raise ValueError("out must have rows of consecutive elements that do not overlap")
-    lo, hi = _span(out)
-    for t in (v for i in inputs if i is not None for v in ((i.codes, i.scales) if isinstance(i, MX4Tensor) else (i,))):
-        if lo < _span(t)[1] and _span(t)[0] < hi:
-            raise ValueError("out must not share memory with an input")
+    refuse_shared(out, "out", *(v for i in inputs for v in ((i.codes, i.scales) if isinstance(i, MX4Tensor) else (i,))))
     _no_grad(out)
     increment_version(out)  # (autograd may have saved it)
     return out, out.stride(0) if shape[0] > 1 else max(1, shape[1])

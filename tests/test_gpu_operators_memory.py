@@ -101,3 +101,47 @@ def test_outputs_of_products_are_seen_by_autograd():
         again = inside.clone()
         call(inside)
         assert torch.equal(inside, again)
+
+
+def test_gradient_may_share_memory_with_the_logits_alone():
+    """Workgroups still read what lies elsewhere: only the logits' own places are each read before they are written."""
+    from lira_amd import distill_topk_loss_and_grad
+    rows, vocab, top = 6, 64, 8
+    g = gen(8)
+    buf = torch.randn(rows + 1, vocab, generator=g, device="cuda")
+    tv, ti = torch.topk(torch.randn(rows, vocab, generator=g, device="cuda"), top, dim=1)
+    ti = ti.int()
+    w, lse = torch.rand(rows, generator=g, device="cuda"), torch.logsumexp(tv, 1)
+    z = buf[:-1]
+    keep = buf.clone()
+    flat = torch.zeros(4 * rows * vocab, device="cuda")
+    cases = [
+        (z, ti, tv, {"grad_out": buf[1:]}),
+        (buf[1:], ti, tv, {"grad_out": buf[:-1]}),
+        (z.flatten()[8:], ti.flatten()[:4], tv.flatten()[:4], {"grad_out": z.flatten()[:-8]}),
+        (buf.as_strided((3, vocab), (2 * vocab, 1)), ti[:3], tv[:3], {"grad_out": buf[:3]}),  # (rows further apart)
+        (z, flat[:rows * top].view(torch.int32).view(rows, top), tv, {"grad_out": flat[:rows * vocab].view(rows, vocab)}),
+        (z, ti, flat[rows * vocab - 1:rows * vocab - 1 + rows * top].view(rows, top), {"grad_out": flat[:rows * vocab].view(rows, vocab)}),
+        (z, ti, tv, {"row_weight": flat[5:5 + rows], "grad_out": flat[:rows * vocab].view(rows, vocab)}),
+        (z, ti, tv, {"teacher_lse": flat[5:5 + rows], "grad_out": flat[:rows * vocab].view(rows, vocab)}),
+    ]
+    for zz, ii, tt, kw in cases:
+        with pytest.raises(ValueError, match="share memory"):
+            distill_topk_loss_and_grad(zz, ii, tt, **kw)
+    assert torch.equal(buf, keep) and not flat.any()
+    # what only looks alike: the logits themselves, the memory behind an input's end, inputs that are copied on the way
+    want, dwant = distill_topk_loss_and_grad(z, ti, tv, teacher_lse=lse, row_weight=w)
+    at = flat[rows * vocab:2 * rows * vocab].view(rows, vocab)
+    flat[:rows * vocab].view(rows, vocab).copy_(z)
+    loss, dz = distill_topk_loss_and_grad(flat[:rows * vocab].view(rows, vocab), ti, tv, teacher_lse=lse, row_weight=w, grad_out=at)
+    assert torch.equal(loss, want) and torch.equal(dz, dwant)
+    t = z.t().contiguous()
+    loss, dz = distill_topk_loss_and_grad(t.t(), ti, tv, teacher_lse=lse, row_weight=w, grad_out=t.view(rows, vocab))
+    assert torch.equal(loss, want) and torch.equal(dz, dwant)
+    own = z.clone()
+    for view in (own, own.view(2, 3, vocab)):
+        own.copy_(z)
+        lead = view.shape[:-1]
+        loss, dz = distill_topk_loss_and_grad(view, ti.view(*lead, top), tv.view(*lead, top), teacher_lse=lse.view(lead),
+                                              row_weight=w.view(lead), grad_out=view)
+        assert torch.equal(loss.flatten(), want) and torch.equal(own, dwant)
