@@ -49,9 +49,11 @@ class MX4Probe(nn.Module):
         super().__init__()
         from .mx4 import mx4_quantize
         state = model.state_dict()
-        missing = [k + e for k in self._LAYERS for e in (".weight", ".bias") if k + e not in state]
-        if missing:
-            raise ValueError(f"MX4Probe needs an MLP_2_Input: the model has no {missing[0]}")
+        names = [k + e for k in self._LAYERS for e in (".weight", ".bias")]
+        missing, more = [k for k in names if k not in state], [k for k in state if k not in names]
+        if missing or more:
+            raise ValueError("MX4Probe needs an MLP_2_Input: the model has " +
+                             (f"no {missing[0]}" if missing else f"{more[0]} as well"))
         with torch.no_grad():
             self.layers = [(mx4_quantize(state[k + ".weight"].float()), state[k + ".bias"].float().clone())
                            for k in self._LAYERS]

@@ -145,3 +145,23 @@ def test_gradient_may_share_memory_with_the_logits_alone():
         loss, dz = distill_topk_loss_and_grad(view, ti.view(*lead, top), tv.view(*lead, top), teacher_lse=lse.view(lead),
                                               row_weight=w.view(lead), grad_out=view)
         assert torch.equal(loss.flatten(), want) and torch.equal(own, dwant)
+
+
+def prober(seed=0, nb=16, d=32):
+    from lira_amd.probing import MLP_2_Input
+    torch.manual_seed(seed)
+    return MLP_2_Input(nb, d, nb).cuda()
+
+
+def test_packed_prober_refuses_a_model_with_more_layers():
+    """Layers that it would leave out: the scores would be another model's."""
+    from lira_amd.probing import MX4Probe
+    deeper = prober()
+    deeper.fc = torch.nn.Sequential(*list(deeper.fc)[:2], torch.nn.Linear(deeper.fc[2].in_features, 16), torch.nn.ReLU(),
+                                    torch.nn.Linear(16, 16), torch.nn.Sigmoid()).cuda()
+    with pytest.raises(ValueError, match="MLP_2_Input"):
+        MX4Probe(deeper)
+    normed = prober()
+    normed.vector_net.add_module("4", torch.nn.BatchNorm1d(normed.vector_net[2].out_features).cuda())
+    with pytest.raises(ValueError, match="MLP_2_Input"):
+        MX4Probe(normed)
