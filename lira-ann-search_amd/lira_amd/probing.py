@@ -35,6 +35,35 @@ class MLP_2_Input(nn.Module):  # noqa: N801 - reference class name, kept for dro
         return self.fc[:-1](torch.cat((self.distance_net(x_dist), self.vector_net(x_vec)), dim=1))
 
 
+class MX4Linear(nn.Module):
+    """A linear layer in 4 bits: packed weights and the bias as buffers, so that ``state_dict()``, ``to()`` and copies
+    take them along.  Runs where they are on the GPU."""
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor):
+        super().__init__()
+        from .mx4 import mx4_quantize
+        with torch.no_grad():
+            w = mx4_quantize(weight.float())
+            self.register_buffer("codes", w.codes)
+            self.register_buffer("scales", w.scales)
+            self.register_buffer("bias", bias.float().clone())
+        self.in_features, self.out_features = w.k, w.n
+        self._packed = w
+
+    def weight(self):
+        """The MX4Tensor of the buffers as they are now (``to()`` and ``load_state_dict(assign=True)`` put others
+        in their place)."""
+        from .mx4 import MX4Tensor
+        w, codes, scales = self._packed, self._buffers["codes"], self._buffers["scales"]
+        if w.codes is not codes or w.scales is not scales:
+            w = self._packed = MX4Tensor(codes, scales, self.in_features)
+        return w
+
+    def forward(self, x: torch.Tensor, activation: str | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+        from .mx4 import mx4_linear
+        return mx4_linear(x, self.weight(), self._buffers["bias"], activation, out=out)
+
+
 class MX4Probe(nn.Module):
     """A trained probing model in 4 bits: the layers of MLP_2_Input (model_probing.py:5-39) with
     packed weights, the activations packed on the way into each (lira_mx4_linear: bias and ReLU or
@@ -47,26 +76,27 @@ class MX4Probe(nn.Module):
 
     def __init__(self, model: nn.Module):
         super().__init__()
-        from .mx4 import mx4_quantize
         state = model.state_dict()
         names = [k + e for k in self._LAYERS for e in (".weight", ".bias")]
         missing, more = [k for k in names if k not in state], [k for k in state if k not in names]
         if missing or more:
             raise ValueError("MX4Probe needs an MLP_2_Input: the model has " +
                              (f"no {missing[0]}" if missing else f"{more[0]} as well"))
-        with torch.no_grad():
-            self.layers = [(mx4_quantize(state[k + ".weight"].float()), state[k + ".bias"].float().clone())
-                           for k in self._LAYERS]
+        # (the names of MLP_2_Input's layers)
+        for net in ("distance_net", "vector_net", "fc"):
+            self.add_module(net, nn.ModuleDict({
+                i: MX4Linear(state[f"{net}.{i}.weight"], state[f"{net}.{i}.bias"]) for i in ("0", "2")}))
 
     @torch.no_grad()
     def forward(self, x_dist: torch.Tensor, x_vec: torch.Tensor) -> torch.Tensor:
-        from .mx4 import mx4_linear
-        (d0, d2, v0, v2, f0, f2), n = self.layers, x_dist.shape[0]
-        nd = d2[0].shape[0]
-        both = torch.empty((n, nd + v2[0].shape[0]), dtype=torch.float32, device=x_dist.device)
-        mx4_linear(mx4_linear(x_dist.float(), *d0, "relu"), *d2, "relu", out=both[:, :nd])
-        mx4_linear(mx4_linear(x_vec.float(), *v0, "relu"), *v2, "relu", out=both[:, nd:])
-        return mx4_linear(mx4_linear(both, *f0, "relu"), *f2, "sigmoid")
+        # (straight to the layers' code: nn.Module's own call takes as long on the host as a layer)
+        d0, d2, v0, v2, f0, f2 = (layer.forward for net in self._modules.values() for layer in net._modules.values())
+        nd = self.distance_net["2"].out_features
+        both = torch.empty((x_dist.shape[0], nd + self.vector_net["2"].out_features), dtype=torch.float32,
+                           device=x_dist.device)
+        d2(d0(x_dist.float(), "relu"), "relu", out=both[:, :nd])
+        v2(v0(x_vec.float(), "relu"), "relu", out=both[:, nd:])
+        return f2(f0(both, "relu"), "sigmoid")
 
 
 class NearestCentroidProbe(nn.Module):

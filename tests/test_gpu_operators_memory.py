@@ -165,3 +165,29 @@ def test_packed_prober_refuses_a_model_with_more_layers():
     normed.vector_net.add_module("4", torch.nn.BatchNorm1d(normed.vector_net[2].out_features).cuda())
     with pytest.raises(ValueError, match="MLP_2_Input"):
         MX4Probe(normed)
+
+
+def test_packed_prober_has_its_weights_in_its_state():
+    from lira_amd.probing import MX4Probe
+    xd, q = torch.randn(50, 16, generator=gen(1), device="cuda"), torch.randn(50, 32, generator=gen(2), device="cuda")
+    probe, other = MX4Probe(prober(0)), MX4Probe(prober(1))
+    want = probe(xd, q)
+    assert not torch.equal(other(xd, q), want)
+    state = probe.state_dict()
+    assert len(state) == 18 and {v.dtype for v in state.values()} == {torch.uint8, torch.float32}
+    other.load_state_dict(state)
+    assert torch.equal(other(xd, q), want)
+    other.load_state_dict({k: v.clone() for k, v in state.items()}, assign=True)
+    assert torch.equal(other(xd, q), want)
+    for again in (copy.deepcopy(probe), pickle.loads(pickle.dumps(probe)), saved(probe)):
+        for v in other.state_dict().values():
+            v.zero_()
+        assert torch.equal(again(xd, q), want)
+    away = copy.deepcopy(probe).cpu()
+    assert all(v.device.type == "cpu" for v in away.state_dict().values())
+    with pytest.raises(ValueError, match="GPU|cpu"):
+        away(xd, q)
+    with pytest.raises(ValueError, match="GPU|cpu"):
+        away(xd.cpu(), q.cpu())
+    assert torch.equal(away.to("cuda")(xd, q), want)
+    assert torch.equal(probe(xd, q), want)
