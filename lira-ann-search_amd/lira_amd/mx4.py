@@ -71,9 +71,10 @@ def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
     """The addresses from t's first element to past its last one."""
-    if t.numel() == 0:
-        return t.data_ptr(), t.data_ptr()
-    return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    at = t.data_ptr()
+    if t.is_contiguous():  # (an empty one is)
+        return at, at + t.nbytes
+    return at, at + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
 def refuse_shared(out: torch.Tensor, name: str, *inputs) -> None:
@@ -98,7 +99,7 @@ class MX4Tensor:
 
     # (what mx4_quantize packs is one buffer, whose two views are made when they are asked for; addresses are
     # read from the tensors at each call, never kept beside them)
-    __slots__ = ("_codes", "_scales", "_buf", "k", "n", "plane_rows")
+    __slots__ = ("_codes", "_scales", "_buf", "k", "n", "plane_rows", "device")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, k: int):
         for t, w, name in ((codes, 64, "codes"), (scales, 4, "scales")):
@@ -121,32 +122,34 @@ class MX4Tensor:
                 scales.clone(memory_format=torch.contiguous_format)
             rows = n
         self._codes, self._scales, self._buf = codes, scales, None
-        self.k, self.n, self.plane_rows = k, n, rows
+        self.k, self.n, self.plane_rows, self.device = k, n, rows, codes.device
 
     @classmethod
     def _of(cls, buf: torch.Tensor, n: int, k: int) -> "MX4Tensor":
         """Of one buffer: the codes, then the scales."""
         t = object.__new__(cls)
         t._codes = t._scales = None
-        t._buf, t.k, t.n, t.plane_rows = buf, k, n, n
+        t._buf, t.k, t.n, t.plane_rows, t.device = buf, k, n, n, buf.device
         return t
 
     def __reduce__(self):
         return _restored, (self.codes, self.scales, self.k)
 
-    @property
-    def device(self) -> torch.device:
-        return (self._buf if self._codes is None else self._codes).device
+    def addresses(self) -> tuple[int, int]:
+        """Of the codes and of the scales."""
+        codes, scales = self._codes, self._scales
+        at = (self._buf if codes is None else codes).data_ptr()
+        if scales is not None:
+            return at, scales.data_ptr()
+        return at, (at if codes is None else self._buf.data_ptr()) + (self.k + 127) // 128 * self.n * 64
 
     @property
     def codes_ptr(self) -> int:
-        return (self._buf if self._codes is None else self._codes).data_ptr()
+        return self.addresses()[0]
 
     @property
     def scales_ptr(self) -> int:
-        if self._scales is None:
-            return self._buf.data_ptr() + (self.k + 127) // 128 * self.n * 64
-        return self._scales.data_ptr()
+        return self.addresses()[1]
 
     @property
     def codes(self) -> torch.Tensor:
@@ -214,7 +217,7 @@ def mx4_quantize(x: torch.Tensor, stream=None) -> MX4Tensor:
     with on(dev, stream):
         x, ld = _rows(x)
         t = MX4Tensor._of(torch.empty(p * n * 68, dtype=torch.uint8, device=dev), n, k)
-        _lib.run("lira_mx4_quantize", x.data_ptr(), DTYPES[x.dtype], n, k, ld, t.codes_ptr, t.scales_ptr, n,
+        _lib.run("lira_mx4_quantize", x.data_ptr(), DTYPES[x.dtype], n, k, ld, *t.addresses(), n,
                  raw_stream(dev.index))
     return t
 
@@ -243,7 +246,7 @@ def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float32, out: torch.
     dev, n = t.device, t.n
     with on(dev, stream):
         out, ld = _out(out, (n, t.k), dtype, dev, t)
-        _lib.run("lira_mx4_dequantize", t.codes_ptr, t.scales_ptr, t.plane_rows, n, t.k, out.data_ptr(), DTYPES[dtype], ld,
+        _lib.run("lira_mx4_dequantize", *t.addresses(), t.plane_rows, n, t.k, out.data_ptr(), DTYPES[dtype], ld,
                  raw_stream(dev.index))
     return out
 
@@ -279,7 +282,7 @@ def mx4_matmul(a: MX4Tensor, b: MX4Tensor, bias: torch.Tensor | None = None, act
     with on(dev, stream):
         bias = None if bias is None else bias.to(torch.float32).contiguous()
         out, ldo = _out(out, (m, n), out_dtype, dev, a, b, bias)
-        _lib.run("lira_mx4_matmul", a.codes_ptr, a.scales_ptr, a.plane_rows, m, b.codes_ptr, b.scales_ptr, b.plane_rows, n, a.k, alpha, _lib.ptr(bias), act, out.data_ptr(),
+        _lib.run("lira_mx4_matmul", *a.addresses(), a.plane_rows, m, *b.addresses(), b.plane_rows, n, a.k, alpha, _lib.ptr(bias), act, out.data_ptr(),
                  DTYPES[out_dtype], ldo, raw_stream(dev.index))
     return out
 
@@ -311,6 +314,6 @@ def mx4_linear(x: torch.Tensor, w: MX4Tensor, bias: torch.Tensor | None = None, 
         bias = None if bias is None else bias.to(torch.float32).contiguous()
         out, ldo = _out(out, (m, n), out_dtype, dev, x, w, bias)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _lib.run("lira_mx4_linear", x.data_ptr(), DTYPES[x.dtype], m, k, ld, w.codes_ptr, w.scales_ptr, w.plane_rows, n, alpha, _lib.ptr(bias), act, out.data_ptr(), DTYPES[out_dtype], ldo, _lib.ptr(ws), need,
+        _lib.run("lira_mx4_linear", x.data_ptr(), DTYPES[x.dtype], m, k, ld, *w.addresses(), w.plane_rows, n, alpha, _lib.ptr(bias), act, out.data_ptr(), DTYPES[out_dtype], ldo, _lib.ptr(ws), need,
                  raw_stream(dev.index))
     return out
