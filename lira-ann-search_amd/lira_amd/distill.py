@@ -21,7 +21,7 @@ import torch
 from torch.autograd.graph import increment_version
 
 from . import _lib
-from .mx4 import DTYPES, check_rows, on, raw_stream, refuse_shared, _rows
+from .mx4 import DTYPES, check_rows, keep_for, on, raw_stream, refuse_shared, _rows
 
 
 def check_device(logits) -> None:
@@ -175,6 +175,7 @@ def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_
     with on(dev, stream):
         z, lead, ids, tv, lse = _entries(logits, top_ids, top_logits, temperature, teacher_lse)
         w = _row_values(row_weight, "row_weight", lead, dev)
+        keep_for(stream, logits, top_ids, top_logits, teacher_lse, row_weight)
         z = _rows(z)[0]  # (perhaps a copy: held until the launch, the head has its address alone)
         if grad_out is None:
             dz = torch.empty(logits.shape, dtype=z.dtype, device=dev)
@@ -185,6 +186,7 @@ def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_
             dz = grad_out
             same = dz.data_ptr() == z.data_ptr() and z.is_contiguous()  # (the logits' own places)
             refuse_shared(dz, "grad_out (but for the logits themselves)", None if same else z, ids, tv, lse, w)
+            keep_for(stream, dz)
             increment_version(dz)  # (autograd may have saved it: the logits' own operation, where it is the logits)
         loss = _forward(_head(z, ids, tv, lse, temperature), dev, None, w, dz)
     return loss if len(lead) == 1 else loss.view(lead), dz

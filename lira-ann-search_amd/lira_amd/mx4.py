@@ -8,7 +8,8 @@ takes 68 bytes, where the reference's fp32 copy (search.cpp:387-403) takes 512.
 * ``mx4_matmul``   act(alpha * A B^T + bias) of two packed arrays
 * ``mx4_linear``   the same with fp32 / bf16 / fp16 rows that are packed on the way
 
-All of them run on the current stream (or ``stream=``), allocate nothing that outlives the call but
+All of them run on the current stream (or ``stream=``: what they read must be ready there; inputs may
+be dropped after the call, results belong to that stream), allocate nothing that outlives the call but
 their results, and can be captured into a graph.  They have no gradient: an input that asks
 for one is refused.
 """
@@ -43,6 +44,17 @@ def on(device: torch.device, stream=None):
             raise ValueError(f"stream is on {stream.device}, the tensors are on {device}")
         return torch.cuda.stream(stream)
     return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def keep_for(stream, *tensors) -> None:
+    """A call on a stream of its own: the memory that it reads or writes belongs to other streams, which must not give
+    it out again before the call is through."""
+    if stream is not None:
+        for t in tensors:
+            if isinstance(t, MX4Tensor):
+                keep_for(stream, t._buf, t._codes, t._scales)
+            elif t is not None:
+                t.record_stream(stream)
 
 
 def check_rows(x, name: str, device=None) -> torch.Tensor:
@@ -215,6 +227,7 @@ def mx4_quantize(x: torch.Tensor, stream=None) -> MX4Tensor:
     p = (k + 127) // 128
     dev = x.device
     with on(dev, stream):
+        keep_for(stream, x)
         x, ld = _rows(x)
         t = MX4Tensor._of(torch.empty(p * n * 68, dtype=torch.uint8, device=dev), n, k)
         _lib.run("lira_mx4_quantize", x.data_ptr(), DTYPES[x.dtype], n, k, ld, *t.addresses(), n,
@@ -246,6 +259,7 @@ def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float32, out: torch.
     dev, n = t.device, t.n
     with on(dev, stream):
         out, ld = _out(out, (n, t.k), dtype, dev, t)
+        keep_for(stream, t, out)
         _lib.run("lira_mx4_dequantize", *t.addresses(), t.plane_rows, n, t.k, out.data_ptr(), DTYPES[dtype], ld,
                  raw_stream(dev.index))
     return out
@@ -280,8 +294,10 @@ def mx4_matmul(a: MX4Tensor, b: MX4Tensor, bias: torch.Tensor | None = None, act
     m, n = a.n, b.n
     dev = a.device
     with on(dev, stream):
+        keep_for(stream, a, b, bias)
         bias = None if bias is None else bias.to(torch.float32).contiguous()
         out, ldo = _out(out, (m, n), out_dtype, dev, a, b, bias)
+        keep_for(stream, out)
         _lib.run("lira_mx4_matmul", *a.addresses(), a.plane_rows, m, *b.addresses(), b.plane_rows, n, a.k, alpha, _lib.ptr(bias), act, out.data_ptr(),
                  DTYPES[out_dtype], ldo, raw_stream(dev.index))
     return out
@@ -310,9 +326,11 @@ def mx4_linear(x: torch.Tensor, w: MX4Tensor, bias: torch.Tensor | None = None, 
     m, n, k, dev = x.shape[0], w.n, w.k, x.device
     need = _linear_workspace(m, n, k)
     with on(dev, stream):
+        keep_for(stream, x, w, bias)
         x, ld = _rows(x)
         bias = None if bias is None else bias.to(torch.float32).contiguous()
         out, ldo = _out(out, (m, n), out_dtype, dev, x, w, bias)
+        keep_for(stream, out)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.run("lira_mx4_linear", x.data_ptr(), DTYPES[x.dtype], m, k, ld, *w.addresses(), w.plane_rows, n, alpha, _lib.ptr(bias), act, out.data_ptr(), DTYPES[out_dtype], ldo, _lib.ptr(ws), need,
                  raw_stream(dev.index))

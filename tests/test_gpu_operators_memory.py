@@ -191,3 +191,63 @@ def test_packed_prober_has_its_weights_in_its_state():
         away(xd.cpu(), q.cpu())
     assert torch.equal(away.to("cuda")(xd, q), want)
     assert torch.equal(probe(xd, q), want)
+
+
+def stream_calls():
+    """name -> (inputs of the current stream, the call that reads them on another one)"""
+    from lira_amd import distill_topk_loss_and_grad, mx4_dequantize, mx4_linear, mx4_matmul, mx4_quantize
+    g = gen(12)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device="cuda")
+
+    rows = 3000  # (of a size that the allocator gives to nothing else here)
+    ids = torch.randint(0, 500, (rows, 70), generator=g, device="cuda")
+    w = mx4_quantize(normal(700, 500))
+    return {
+        "quantize": ([normal(rows, 500)], lambda s, x: mx4_quantize(x, stream=s)),
+        "quantize columns": ([normal(500, rows)], lambda s, x: mx4_quantize(x.t(), stream=s)),
+        "dequantize": ([mx4_quantize(normal(rows, 500))], lambda s, t: mx4_dequantize(t, stream=s)),
+        "dequantize out": ([normal(700, 500)], lambda s, out: w.dequantize(out=out, stream=s)),
+        "linear": ([normal(rows, 500), mx4_quantize(normal(700, 500)), normal(700).half()],
+                   lambda s, x, w, b: mx4_linear(x, w, b, stream=s)),
+        "matmul": ([mx4_quantize(normal(rows, 500)), mx4_quantize(normal(700, 500)), normal(700)],
+                   lambda s, a, b, c: mx4_matmul(a, b, c, stream=s)),
+        "linear out": ([normal(rows, 700)], lambda s, out, x=normal(rows, 500): mx4_linear(x, w, out=out, stream=s)),
+        "distill": ([normal(rows, 500), ids, normal(rows, 70), normal(rows), normal(rows)],
+                    lambda s, z, i, t, lse, wt: distill_topk_loss_and_grad(z, i, t, 1.0, lse, wt, stream=s)),
+        "distill out": ([normal(rows, 500)], lambda s, dz, z=normal(rows, 500), t=normal(rows, 70):
+                        distill_topk_loss_and_grad(z, ids, t, grad_out=dz, stream=s)),
+    }
+
+
+@pytest.mark.parametrize("name", ["quantize", "quantize columns", "dequantize", "dequantize out", "linear", "matmul", "linear out",
+                                  "distill", "distill out"])
+def test_memory_read_on_another_stream_is_not_given_out_again(name):
+    """An input that is dropped right after the call: its stream's allocator must not hand its memory out while the
+    other stream has work that reads it (looked at by address: nothing writes there)."""
+    from lira_amd import MX4Tensor
+    side = torch.cuda.Stream()
+    inputs, call = stream_calls()[name]
+    call(side, *inputs)  # (its kernels are loaded)
+    torch.cuda.synchronize()
+    inputs, call = stream_calls()[name]
+    side.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(50_000_000)  # (half a second at most; the call waits behind it)
+    kept = []
+    result = call(side, *inputs)
+    held = [b for t in inputs for b in ((t._buf,) if isinstance(t, MX4Tensor) and t._buf is not None else
+                                        (t.codes, t.scales) if isinstance(t, MX4Tensor) else (t,))]
+    spans = [(b.untyped_storage().data_ptr(), b.untyped_storage().nbytes()) for b in held]
+    del inputs, call, held
+    for at, size in spans:
+        kept += [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(3)]
+    pending = not side.query()
+    for new in kept:
+        for at, size in spans:
+            assert new.data_ptr() + new.numel() <= at or at + size <= new.data_ptr()
+    assert pending  # (else the test has looked too late)
+    torch.cuda.synchronize()
+    del result
