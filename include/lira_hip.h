@@ -390,10 +390,10 @@ int lira_mx4_linear(const void *x, int dtype, int64_t m, int64_t k, int64_t ldx,
  *   loss[r] = T^2 sum_{p_j > 0} p_j (log p_j - log q_ids[j])
  *   dz[r,v] = row_scale[r * scale_stride] T (s q_v - sum_{j: ids[j] = v} p_j)
  * ids < 0 are unused entries; an id may occur more than once.  A row in which no
- * entry counts (all unused, or of p = 0) has loss 0 and gradient 0, whatever its
- * logits.  z_v = -inf is a masked output: q_v = 0 (the loss is +inf where an entry
- * of p > 0 names it).  NaN or +inf among the z, NaN among the used entries, or an
- * id >= vocab makes the row's loss and gradient NaN.
+ * entry counts (all unused, or of p = 0, as teacher = -inf is whatever L) has loss
+ * 0 and gradient 0, whatever its logits.  z_v = -inf is a masked output: q_v = 0
+ * (the loss is +inf where an entry of p > 0 names it).  NaN or +inf among the z, NaN
+ * among the used entries, or an id >= vocab makes the row's loss and gradient NaN.
  *   z, dz     dtype, (rows, vocab), row strides ldz / ldd elements, any
  *             alignment; dz may be z itself (ldd = ldz), else must not overlap it
  *   ids       int32 or int64 (ids_bits), (rows, top); teacher fp32 (rows, top);

@@ -227,8 +227,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
             const int j = i * 64 + lane;
             bad |= id[i] == INT32_MAX;
             lp[i] = fmaf(tv[i] - tm, c, -L2);
-            p[i] = id[i] < 0 ? 0.0f : ex2(lp[i]);
-            if (a.teacher_lse && id[i] >= 0 && tv[i] != -INFINITY && p[i] != p[i]) bad = true;
+            // (an entry of -inf is 0 whatever L: the logsumexp of a teacher row that is masked whole is -inf too)
+            p[i] = id[i] < 0 || tv[i] == -INFINITY ? 0.0f : ex2(lp[i]);
             any |= !(p[i] == 0.0f);
             tot += p[i];
             xe[i] = 0.0f;
