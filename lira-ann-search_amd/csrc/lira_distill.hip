@@ -131,8 +131,12 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
     static_assert(NT >= 64 && (G == 1 || NW == 1), "a group is a wave or a workgroup");
     __shared__ float sm[G][NW], ss[G][NW];
     __shared__ float s_p[G][kEntries ? KM : 1], s_x[G][kEntries ? KM : 1];
-    __shared__ int s_id[G][kEntries ? KM : 1], s_next[G][kEntries ? KM : 1], s_head[G][kDz ? NT : 1];
+    __shared__ __attribute__((aligned(16))) int s_id[G][kEntries ? KM : 1];
+    __shared__ int s_next[G][kEntries ? KM : 1], s_head[G][kDz ? NT : 1];
+    constexpr int NC = NT < 256 ? NT : 256;
+    __shared__ int s_count[G][kDz ? NC : 1];  // entries of the lists (of the threads u, u + 256, .. together)
     __shared__ float s_tot[G][2];
+    __shared__ int s_many[G];
     const int gi = G == 1 ? 0 : threadIdx.x >> 6, u = G == 1 ? threadIdx.x : threadIdx.x & 63;
     const int lane = threadIdx.x & 63, w = G == 1 ? threadIdx.x >> 6 : 0;
     auto sync = [&]() {
@@ -193,11 +197,16 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
     }
     const float x1 = single ? D::up(z[at1]) : -INFINITY;
 
+    // Entries of a list that is walked, which takes the square of its length in steps that wait for each other; where
+    // one is longer, the row's threads go over all entries for each id (256 x 4096, top 1024: ids apart 35 us and 42;
+    // of one id 137 ms walked, 0.15 gone over; 4096 x 1024, top 64, padded with id 0: 700 us and 15).
+    const int most = max(8, a.top / 16);
+
     // ------------------------------------------------------------ entries
     // of the first wave: p, log2 p and the z they name; in LDS p, z, the id and the owner's list
     float p[J], lp[J], xe[J];
     float tot = 0.0f;
-    bool bad = false, any = false;
+    bool bad = false, any = false, many = false;
     if (first) {
         float L2;
         float tm = -INFINITY;
@@ -220,6 +229,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
         if (kDz) {
 #pragma unroll
             for (int i = 0; i < NW; ++i) s_head[gi][i * 64 + lane] = -1;
+#pragma unroll
+            for (int i = 0; i < NC / 64; ++i) s_count[gi][i * 64 + lane] = 0;
             __builtin_amdgcn_wave_barrier();
         }
 #pragma unroll
@@ -243,13 +254,18 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
                 s_id[gi][j] = id[i];
                 const int e = id[i] - h, v = e / E;
                 const bool lone = e < 0 || e >= shift;
-                if (real && (lone ? singles != 0 : v >= v0 && v < v1))
-                    s_next[gi][j] = atomicExch(&s_head[gi][!lone ? (v - v0) % NT : e < 0 ? id[i] : id[i] - shift], j);
+                // (an entry of p = 0 changes nothing: lists padded with id 0 would all be one thread's)
+                if (real && !(p[i] == 0.0f) && (lone ? singles != 0 : v >= v0 && v < v1)) {
+                    const int owner = !lone ? (v - v0) % NT : e < 0 ? id[i] : id[i] - shift;
+                    s_next[gi][j] = atomicExch(&s_head[gi][owner], j);
+                    many |= atomicAdd(&s_count[gi][owner % NC], 1) >= most;
+                }
             }
         }
         tot = wave_sum(tot);
         if (__any(bad)) tot = NAN;
         any = __any(any) || tot != tot;
+        many = __any(many);
     }
     if (MODE == kPart && slice == 0 && w == 0) {
         for (int j = lane; j < a.top; j += 64) {
@@ -302,7 +318,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
         }
     }
     if (NW > 1 && kStats && lane == 0) sm[gi][w] = m, ss[gi][w] = s;
-    if (NW > 1 && first && lane == 0) s_tot[gi][0] = tot, s_tot[gi][1] = any ? 1.0f : 0.0f;
+    if (NW > 1 && first && lane == 0) s_tot[gi][0] = tot, s_tot[gi][1] = any ? 1.0f : 0.0f, s_many[gi] = many;
     sync();
     if (NW > 1 && kEntries && !first) tot = s_tot[gi][0], any = s_tot[gi][1] != 0.0f;
     auto join = [&](float m1, float s1) {
@@ -386,22 +402,49 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void k_distill(DistillArgs a) 
         }
         if (single) dz[at1] = D::down(any ? f * ex2(fmaf(x1 - m, c, -l2)) : 0.0f);
         if (!any || tot != tot) return;
-        // this thread's entries: of several with one id the first adds up all, in their order
-        for (int j = s_head[gi][u]; j >= 0; j = s_next[gi][j]) {
-            const int k = s_id[gi][j];
-            bool lead = true;
-            for (int i = s_head[gi][u]; i >= 0; i = s_next[gi][i]) lead &= !(s_id[gi][i] == k && i < j);
-            if (!lead) continue;
-            float sum = 0.0f;
-            for (int at = j; at < KM;) {
-                sum += s_p[gi][at];
-                int next = KM;
-                for (int i = s_head[gi][u]; i >= 0; i = s_next[gi][i])
-                    if (s_id[gi][i] == k && i > at && i < next) next = i;
-                at = next;
-            }
+        auto place = [&](int j, int k, float sum) {
             const float q = ex2(fmaf(s_x[gi][j] - m, c, -l2));
             dz[k] = D::down(g * (tot * q - sum));
+        };
+        // this thread's entries: of several with one id the first adds up all, in their order
+        if (s_head[gi][u] < 0) return;
+        if (NW > 1) many = s_many[gi];  // (read here: kept in a register from the barrier on, 131071 outputs take 1.5 % more)
+        if (__builtin_expect(!many, 1)) {
+            for (int j = s_head[gi][u]; j >= 0; j = s_next[gi][j]) {
+                const int k = s_id[gi][j];
+                bool lead = true;
+                for (int i = s_head[gi][u]; i >= 0; i = s_next[gi][i]) lead &= !(s_id[gi][i] == k && i < j);
+                if (!lead) continue;
+                float sum = 0.0f;
+                for (int at = j; at < KM;) {
+                    sum += s_p[gi][at];
+                    int next = KM;
+                    for (int i = s_head[gi][u]; i >= 0; i = s_next[gi][i])
+                        if (s_id[gi][i] == k && i > at && i < next) next = i;
+                    at = next;
+                }
+                place(j, k, sum);
+            }
+            return;
+        }
+        // a long list: 16 entries at a time, and those found are struck out (an id has one owner: no other thread
+        // looks for it)
+        for (int j = s_head[gi][u]; j >= 0; j = s_next[gi][j]) {
+            const int k = s_id[gi][j];
+            if (k < 0) continue;
+            float sum = 0.0f;
+            for (int i = 0; i < a.top; i += 16) {
+                i32x4 v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const i32x4 *>(&s_id[gi][i + e * 4]);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (v[e / 4][e % 4] == k) {
+                        sum += s_p[gi][i + e];
+                        s_id[gi][i + e] = -1;
+                    }
+            }
+            place(j, k, sum);
         }
     }
 }

@@ -53,3 +53,18 @@ def test_entries_padded_with_a_logit_of_minus_infinity(rows, vocab, top):
     unused = both(z, ti.masked_fill(gone, -1), tv, 2.0)
     for a, b in zip(padded, unused):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("rows,vocab,top,ids", [(3, 2000, 1024, 1), (3, 100000, 1024, 1), (5, 4000, 64, 1), (9, 4000, 700, 3),
+                                                (4, 70000, 1024, 8), (600, 1000, 64, 2), (4, 300000, 1024, 1000)])
+def test_many_entries_of_one_output(rows, vocab, top, ids):
+    """All entries name the same few outputs, next to each other: one thread stores them all."""
+    g = torch.Generator(device="cuda").manual_seed(top + ids)
+    z = torch.randn(rows, vocab, generator=g, device="cuda")
+    ti = vocab // 3 + torch.randint(0, ids, (rows, top), generator=g, device="cuda")
+    tv = torch.randn(rows, top, generator=g, device="cuda")
+    loss, grad, tl, tg = ref(z, ti, tv, 1.0)
+    # (an output named up to `top` times: that many additions more, of at most 1 in all)
+    for got, dz in both(z, ti, tv, 1.0):
+        check_loss(got, loss, tl + loss.abs() * top * 2.0 ** -24)
+        check_grad(dz, grad, tg + top * 2.0 ** -24)
