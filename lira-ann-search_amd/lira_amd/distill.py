@@ -98,6 +98,16 @@ def _forward(head, dev, stats, row_weight, dz):
     return loss
 
 
+_KINDS = {**DTYPES, torch.int32: 32, torch.int64: 64}
+
+
+def _same(t: torch.Tensor, shape: tuple, kind: int, device: torch.device) -> torch.Tensor:
+    """A tensor that the backward pass reads by address: as it was saved, but for its layout."""
+    if t.shape != shape or _KINDS.get(t.dtype) != kind or not t.is_cuda or t.device != device:
+        raise RuntimeError(f"distill_topk_loss: a saved tensor came back as {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.contiguous()
+
+
 class _Loss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, ids, tv, lse, t, reduction):
@@ -121,10 +131,16 @@ class _Loss(torch.autograd.Function):
     def backward(ctx, g):
         if torch.is_grad_enabled():
             raise RuntimeError("distill_topk_loss has no second derivative (create_graph=True)")
-        # (not always the tensors of the forward pass: hooks may have moved them.  The engine has made their device and
-        # the forward pass's stream the current ones.)
+        # (not always the tensors of the forward pass: hooks may have moved them, or laid them out otherwise.  The engine
+        # has made their device and the forward pass's stream the current ones.)
         z, ids, tv, lse, stats = ctx.saved_tensors
         dtype, rows, vocab, ld, bits, top, t = ctx.sizes
+        if z.shape != (rows, vocab) or DTYPES.get(z.dtype) != dtype or not z.is_cuda:
+            raise RuntimeError(f"distill_topk_loss: the logits came back as {tuple(z.shape)} {z.dtype} on {z.device}")
+        ids = _same(ids, (rows, top), bits, z.device)
+        tv, stats = _same(tv, (rows, top), _lib.LIRA_DTYPE_F32, z.device), _same(stats, (rows, 4), _lib.LIRA_DTYPE_F32, z.device)
+        if lse is not None:
+            lse = _same(lse, (rows,), _lib.LIRA_DTYPE_F32, z.device)
         if z.stride() != (ld, 1):
             z, ld = _rows(z)
         if ctx.factor is not None:

@@ -68,3 +68,44 @@ def test_many_entries_of_one_output(rows, vocab, top, ids):
     for got, dz in both(z, ti, tv, 1.0):
         check_loss(got, loss, tl + loss.abs() * top * 2.0 ** -24)
         check_grad(dz, grad, tg + top * 2.0 ** -24)
+
+
+def test_what_hooks_bring_back_in_another_layout():
+    """Saved-tensor hooks may return the same values in tensors that are laid out otherwise."""
+    from lira_amd import distill_topk_loss
+    z, ti, tv, w = make(30, 800, 9, "fp32")
+    lse = torch.logsumexp(z, 1)
+    z.requires_grad_(True)
+
+    def step():
+        (g,) = torch.autograd.grad(distill_topk_loss(z, ti, tv, 2.0, teacher_lse=lse, reduction="none"), z, w)
+        return g
+
+    def spread(t):
+        return torch.stack((t, t), -1)[..., 0]  # (every second element of twice the memory)
+
+    want = step()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
+        got = step()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("which", range(5))
+@pytest.mark.parametrize("change", [lambda t: t.half(), lambda t: t[:-1], lambda t: t.cpu(), lambda t: t.flatten()])
+def test_what_hooks_bring_back_as_another_tensor(which, change):
+    """Another type, size or device than was saved: refused, not read as if it were the same."""
+    from lira_amd import distill_topk_loss
+    z, ti, tv, _ = make(30, 800, 9, "fp32")
+    lse = torch.logsumexp(z, 1)
+    if which == 3 and change(lse).shape == lse.shape and change(lse).dtype == lse.dtype and change(lse).is_cuda:
+        pytest.skip("this change leaves a vector as it is")
+    z.requires_grad_(True)
+    count = iter(range(5))  # (saved in the order logits, ids, teacher, its logsumexp, statistics)
+
+    def unpack(t):
+        return change(t) if next(count) == which else t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        loss = distill_topk_loss(z, ti, tv, 2.0, teacher_lse=lse)
+    with pytest.raises(RuntimeError, match="came back"):
+        loss.backward()
