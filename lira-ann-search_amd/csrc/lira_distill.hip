@@ -472,14 +472,28 @@ __global__ __launch_bounds__(1024) void k_distill_reduce(const float *loss, cons
     out[1] = f;
 }
 
+// A launch has fewer than 2^32 threads: more rows take another one.
 template <class D, int NT, int NV, int KM, Mode MODE>
-static int launch(const DistillArgs &a, hipStream_t st) {
-    constexpr int G = NT < 256 ? 256 / NT : 1;
-    const int64_t groups = a.rows * (MODE == kPart || MODE == kJoin || MODE == kGrad ? a.slices : 1);
-    if ((groups + G - 1) / G > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "distill: too many rows for one launch");
-    hipLaunchKernelGGL((k_distill<D, NT, NV, KM, MODE>), dim3((unsigned)((groups + G - 1) / G)), dim3(NT < 256 ? 256 : NT),
-                       0, st, a);
-    LIRA_HIP_TRY(hipGetLastError());
+static int launch(DistillArgs a, hipStream_t st) {
+    constexpr int G = NT < 256 ? 256 / NT : 1, threads = NT < 256 ? 256 : NT;
+    const int64_t each = MODE == kPart || MODE == kJoin || MODE == kGrad ? a.slices : 1;  // groups a row
+    const int64_t most = (int64_t)(UINT32_MAX / threads) * G / each;
+    for (int64_t left = a.rows; left > 0;) {
+        const int64_t n = a.rows = std::min(left, most);
+        hipLaunchKernelGGL((k_distill<D, NT, NV, KM, MODE>), dim3((unsigned)((n * each + G - 1) / G)), dim3(threads), 0, st, a);
+        LIRA_HIP_TRY(hipGetLastError());
+        if ((left -= n) == 0) break;
+        a.z = (const typename D::T *)a.z + n * a.ldz;
+        a.ids = (const char *)a.ids + n * a.top * (a.ids64 ? 8 : 4);
+        a.tv += n * a.top;
+        if (a.teacher_lse) a.teacher_lse += n;
+        if (a.row_scale) a.row_scale += n * a.scale_stride;
+        if (a.loss) a.loss += n;
+        if (a.stats) a.stats += n * 4;
+        if (a.dz) a.dz = (typename D::T *)a.dz + n * a.ldd;
+        if (a.part) a.part += n * a.slices;
+        if (a.xs) a.xs += n * a.top;
+    }
     return LIRA_OK;
 }
 
@@ -554,7 +568,7 @@ static int check_distill(const DistillArgs &a, int dtype, int ids_bits) {
     if (a.row_scale && (a.scale_stride < 0 || a.scale_stride > 1))
         return fail(LIRA_EINVAL, "scale_stride must be 0 or 1");
     if (a.vocab >= INT32_MAX) return fail(LIRA_EUNSUPPORTED, "vocab must be less than 2147483647");
-    if (a.rows > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "too many rows for one launch");
+    if (a.rows > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "too many rows");
     if (a.rows > 0 && (!a.z || !a.ids || !a.tv)) return fail(LIRA_EINVAL, "NULL buffer");
     return LIRA_OK;
 }

@@ -592,29 +592,34 @@ static int check_packed(const void *codes, const void *scales, int64_t rows, int
     return LIRA_OK;
 }
 static int check_grid(int64_t blocks, const char *what) {
-    return blocks > INT32_MAX ? fail(LIRA_EUNSUPPORTED, std::string(what) + ": too many rows for one launch") : LIRA_OK;
+    return blocks > INT32_MAX ? fail(LIRA_EUNSUPPORTED, std::string(what) + ": too many rows") : LIRA_OK;
 }
+// A launch has fewer than 2^32 threads along x: the rows that workgroups of 256 threads and `each` rows can take.
+static constexpr int64_t launch_rows_most(int each) { return (int64_t)(UINT32_MAX / 256) * each; }
 
 template <class D>
 static int quantize(const void *x, int64_t n, int64_t k, int64_t ld, uint8_t *codes, uint8_t *scales,
                     int64_t plane_rows, hipStream_t st) {
     typedef typename D::T T;
     const bool vec = ((uintptr_t)x & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
-    const dim3 g((unsigned)((n + 15) / 16), (unsigned)planes_of(k));
     // What the last kernel left of x may be in the caches; of x several times their size nothing is, and its
     // loads would push out the packed rows (1M x 128, packed and read back: 196 us, 184 with ONCE;
     // 10000 x 128 packed 2.9 us, 3.7 with it).
     const bool once = n * k * (int64_t)sizeof(T) >= (int64_t)128 << 20;
-    if (!vec)
-        hipLaunchKernelGGL((k_mx4_quantize<D, false, false>), g, dim3(256), 0, st, (const T *)x, n, k, ld, codes, scales,
-                           plane_rows);
-    else if (once)
-        hipLaunchKernelGGL((k_mx4_quantize<D, true, true>), g, dim3(256), 0, st, (const T *)x, n, k, ld, codes, scales,
-                           plane_rows);
-    else
-        hipLaunchKernelGGL((k_mx4_quantize<D, true, false>), g, dim3(256), 0, st, (const T *)x, n, k, ld, codes, scales,
-                           plane_rows);
-    LIRA_HIP_TRY(hipGetLastError());
+    constexpr int64_t most = launch_rows_most(16);
+    for (int64_t r = 0; r < n; r += most) {
+        const int64_t rows = std::min(n - r, most);
+        const dim3 g((unsigned)((rows + 15) / 16), (unsigned)planes_of(k));
+        const T *at = (const T *)x + r * ld;
+        uint8_t *c = codes + r * 64, *s = scales + r * 4;
+        if (!vec)
+            hipLaunchKernelGGL((k_mx4_quantize<D, false, false>), g, dim3(256), 0, st, at, rows, k, ld, c, s, plane_rows);
+        else if (once)
+            hipLaunchKernelGGL((k_mx4_quantize<D, true, true>), g, dim3(256), 0, st, at, rows, k, ld, c, s, plane_rows);
+        else
+            hipLaunchKernelGGL((k_mx4_quantize<D, true, false>), g, dim3(256), 0, st, at, rows, k, ld, c, s, plane_rows);
+        LIRA_HIP_TRY(hipGetLastError());
+    }
     return LIRA_OK;
 }
 
@@ -624,12 +629,18 @@ static int dequantize(const uint8_t *codes, const uint8_t *scales, int64_t plane
     typedef typename D::T T;
     constexpr int R = 256 / (kPlane / (16 / (int)sizeof(T)));  // rows of a workgroup
     const bool vec = ((uintptr_t)out & 15) == 0 && (ld * sizeof(T)) % 16 == 0;
-    const dim3 g((unsigned)((n + R - 1) / R), (unsigned)planes_of(k));
-    if (vec)
-        hipLaunchKernelGGL((k_mx4_dequantize<D, true>), g, dim3(256), 0, st, codes, scales, plane_rows, n, k, (T *)out, ld);
-    else
-        hipLaunchKernelGGL((k_mx4_dequantize<D, false>), g, dim3(256), 0, st, codes, scales, plane_rows, n, k, (T *)out, ld);
-    LIRA_HIP_TRY(hipGetLastError());
+    constexpr int64_t most = launch_rows_most(R);
+    for (int64_t r = 0; r < n; r += most) {
+        const int64_t rows = std::min(n - r, most);
+        const dim3 g((unsigned)((rows + R - 1) / R), (unsigned)planes_of(k));
+        const uint8_t *c = codes + r * 64, *s = scales + r * 4;
+        T *at = (T *)out + r * ld;
+        if (vec)
+            hipLaunchKernelGGL((k_mx4_dequantize<D, true>), g, dim3(256), 0, st, c, s, plane_rows, rows, k, at, ld);
+        else
+            hipLaunchKernelGGL((k_mx4_dequantize<D, false>), g, dim3(256), 0, st, c, s, plane_rows, rows, k, at, ld);
+        LIRA_HIP_TRY(hipGetLastError());
+    }
     return LIRA_OK;
 }
 
@@ -645,7 +656,6 @@ static int launch_tile(const Product &p, hipStream_t st, const Rows &r = {nullpt
     const int steps = (p.planes + PS - 1) / PS, slots = std::min(SLOTS, steps) * PS * C::kPlaneBytes;
     const int bytes = std::min<int>(C::kBytes, std::max<int>(slots, C::template epilogue_bytes<D>()));
     const int64_t tn = (p.n + TN - 1) / TN, tm = (p.m + TM - 1) / TM;
-    if (tn * tm > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "product: too many tiles for one launch");
     hipLaunchKernelGGL((k_mx4_tile<TN, TM, WN, WM, WK, SLOTS, PS, D, X>), dim3((unsigned)(tn * tm)), dim3(C::NW * 64), bytes, st, p,
                        r, (int)tn, (int)tm);
     LIRA_HIP_TRY(hipGetLastError());
@@ -698,26 +708,26 @@ static int linear_rows(const Product &p, const Rows &r, hipStream_t st) {
 // of many planes (37 x 11111 x 5000: 11.8 us by the third, 13.3 by the fifth); the others are small enough in LDS for
 // two or more a unit (37 x 300000 x 128: 11 us by the sixth, 28 by the third).
 static const struct {
-    int tn, tm;
+    int tn, tm, waves;
     float start, plane, tile, step;
 } kTiles[] = {
-    {32, 32, 3.136f, 0.043f, 0.875f, 0.065f},
-    {64, 32, 3.796f, 0.017f, 1.108f, 0.138f},
-    {64, 64, 3.794f, 0.033f, 1.852f, 0.170f},
-    {64, 32, 2.975f, 0.133f, 0.417f, 0.073f},
-    {64, 64, 3.127f, 0.149f, 0.473f, 0.096f},
-    {128, 64, 3.607f, 0.179f, 0.699f, 0.160f},
-    {128, 128, 3.989f, 0.215f, 1.542f, 0.246f},
-    {256, 256, 3.441f, 0.340f, 6.660f, 0.784f},
+    {32, 32, 8, 3.136f, 0.043f, 0.875f, 0.065f},
+    {64, 32, 8, 3.796f, 0.017f, 1.108f, 0.138f},
+    {64, 64, 8, 3.794f, 0.033f, 1.852f, 0.170f},
+    {64, 32, 4, 2.975f, 0.133f, 0.417f, 0.073f},
+    {64, 64, 4, 3.127f, 0.149f, 0.473f, 0.096f},
+    {128, 64, 4, 3.607f, 0.179f, 0.699f, 0.160f},
+    {128, 128, 4, 3.989f, 0.215f, 1.542f, 0.246f},
+    {256, 256, 8, 3.441f, 0.340f, 6.660f, 0.784f},
 };
-static int tile_for(const Product &p) {
+static int tile_for(int64_t m, int64_t n, int64_t planes) {
     int best = 0;
     float least = INFINITY;
     for (int i = 0; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
         const auto &t = kTiles[i];
-        const int64_t tiles = ((p.n + t.tn - 1) / t.tn) * ((p.m + t.tm - 1) / t.tm);
+        const int64_t tiles = ((n + t.tn - 1) / t.tn) * ((m + t.tm - 1) / t.tm);
         const float load = 0.5f * ((float)((tiles + 255) / 256) + (float)tiles / 256.0f);
-        const float us = t.start + p.planes * t.plane + load * (t.tile + p.planes * t.step);
+        const float us = t.start + planes * t.plane + load * (t.tile + planes * t.step);
         if (us < least) least = us, best = i;
     }
     return best;
@@ -730,7 +740,7 @@ static int product(const Product &p, hipStream_t st) {
         if (split_planes(p)) return launch_rows<F32, D, 1, 8, false, false>(p, r, st);
         return launch_rows<F32, D, 2, 1, false, false>(p, r, st);
     }
-    switch (tile_for(p)) {
+    switch (tile_for(p.m, p.n, p.planes)) {
     case 0: return launch_tile<32, 32, 1, 2, 4, 4, 4, D>(p, st);
     case 1: return launch_tile<64, 32, 2, 1, 4, 4, 4, D>(p, st);
     case 2: return launch_tile<64, 64, 2, 1, 4, 4, 4, D>(p, st);
@@ -768,13 +778,19 @@ static int product(const Product &p, int out_dtype, hipStream_t st) {
     return product<F16>(p, st);
 }
 
-static int check_product(int64_t m, int64_t n, int act, const void *out, int out_dtype, int64_t ldo) {
+static int check_product(int64_t m, int64_t n, int64_t k, int act, const void *out, int out_dtype, int64_t ldo) {
     if (!dtype_ok(out_dtype)) return fail(LIRA_EINVAL, "unknown dtype");
     if (act < LIRA_ACT_NONE || act > LIRA_ACT_SIGMOID) return fail(LIRA_EINVAL, "unknown activation");
     if (ldo < n) return fail(LIRA_EINVAL, "ldo must be at least n");
     if (m > 0 && n > 0 && !out) return fail(LIRA_EINVAL, "NULL buffer");
-    if (m > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "product: too many rows for one launch");
-    return check_grid((n + 15) / 16, "product");
+    if (m > INT32_MAX) return fail(LIRA_EUNSUPPORTED, "product: too many rows");
+    if (int rc = check_grid((n + 15) / 16, "product")) return rc;
+    if (m > 16) {  // (rows that their tiles pack have few)
+        const auto &t = kTiles[tile_for(m, n, planes_of(k))];
+        if (((n + t.tn - 1) / t.tn) * ((m + t.tm - 1) / t.tm) > (int64_t)(UINT32_MAX / (t.waves * 64)))
+            return fail(LIRA_EUNSUPPORTED, "product: too many tiles for one launch, which has fewer than 2^32 threads");
+    }
+    return LIRA_OK;
 }
 
 }  // namespace lira
@@ -816,7 +832,7 @@ int lira_mx4_matmul(const uint8_t *a_codes, const uint8_t *a_scales, int64_t a_p
                     float alpha, const float *bias, int act, void *out, int out_dtype, int64_t ldo, void *stream) {
     if (int rc = check_packed(a_codes, a_scales, m, a_plane_rows, k)) return rc;
     if (int rc = check_packed(b_codes, b_scales, n, b_plane_rows, k)) return rc;
-    if (int rc = check_product(m, n, act, out, out_dtype, ldo)) return rc;
+    if (int rc = check_product(m, n, k, act, out, out_dtype, ldo)) return rc;
     if (m == 0 || n == 0) return LIRA_OK;
     hipStream_t st = (hipStream_t)stream;
     const Product p = {a_codes, a_scales, b_codes, b_scales, a_plane_rows, b_plane_rows, m, n, ldo,
@@ -838,7 +854,7 @@ int lira_mx4_linear(const void *x, int dtype, int64_t m, int64_t k, int64_t ldx,
     if (int rc = check_packed(b_codes, b_scales, n, b_plane_rows, k)) return rc;
     if (m < 0) return fail(LIRA_EINVAL, "bad shape");
     if (ldx < k) return fail(LIRA_EINVAL, "ldx must be at least k");
-    if (int rc = check_product(m, n, act, out, out_dtype, ldo)) return rc;
+    if (int rc = check_product(m, n, k, act, out, out_dtype, ldo)) return rc;
     if (m == 0 || n == 0) return LIRA_OK;
     if (!x) return fail(LIRA_EINVAL, "NULL buffer");
     size_t need = 0;
