@@ -389,6 +389,7 @@ int lira_mx4_linear(const void *x, int dtype, int64_t m, int64_t k, int64_t ldx,
  *   log q_v = z_v / T - logsumexp_v(z_v / T)
  *   loss[r] = T^2 sum_{p_j > 0} p_j (log p_j - log q_ids[j])
  *   dz[r,v] = row_scale[r * scale_stride] T (s q_v - sum_{j: ids[j] = v} p_j)
+ * T is within 1.1e-19 .. 1.8e19 (its square is a factor of the loss).
  * ids < 0 are unused entries; an id may occur more than once.  A row in which no
  * entry counts (all unused, or of p = 0, as teacher = -inf is whatever L) has loss
  * 0 and gradient 0, whatever its logits.  z_v = -inf is a masked output: q_v = 0

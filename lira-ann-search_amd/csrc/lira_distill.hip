@@ -24,6 +24,7 @@
 // into a list of the thread that stores its place (LDS); that thread stores the place once more
 // after its vectors -- its own stores to one address stay in order, so no barrier waits for them.
 #include <algorithm>
+#include <cfloat>
 #include <string>
 
 #include "lira_device.hpp"
@@ -565,6 +566,8 @@ static int check_distill(const DistillArgs &a, int dtype, int ids_bits) {
     if (a.ldz < a.vocab || (a.dz && a.ldd < a.vocab)) return fail(LIRA_EINVAL, "row strides must be at least vocab");
     if (!(a.t > 0.0f) || !(a.t < INFINITY) || !(kLog2e / a.t < INFINITY))
         return fail(LIRA_EINVAL, "temperature must be positive and finite");
+    if (!(a.t * a.t < INFINITY) || a.t * a.t < FLT_MIN)  // (the loss's factor)
+        return fail(LIRA_EINVAL, "temperature must have a square that fp32 holds, 1.1e-19 to 1.8e19");
     if (a.row_scale && (a.scale_stride < 0 || a.scale_stride > 1))
         return fail(LIRA_EINVAL, "scale_stride must be 0 or 1");
     if (a.vocab >= INT32_MAX) return fail(LIRA_EUNSUPPORTED, "vocab must be less than 2147483647");

@@ -17,6 +17,14 @@ def test_products_of_more_tiles_than_a_launch_has_threads(m, n, k):
     assert "too many tiles" in lib.lira_last_error().decode()
 
 
+@pytest.mark.parametrize("t,ok", [(1e-20, False), (1e-19, False), (1.1e-19, True), (1.8e19, True), (1.9e19, False), (1e30, False)])
+def test_temperatures_whose_square_leaves_fp32(t, ok):
+    """The loss has the factor T^2: past fp32's end it was NaN or infinite, and 0 below its smallest number."""
+    lib = _lib.load()
+    rc = lib.lira_distill_topk(A, 0, 0, 100, 100, A, 32, A, 5, t, None, A, None, None, 0, None, 0, None, 0, None)  # (of no rows)
+    assert (rc == 0) if ok else (rc == -1 and "square" in lib.lira_last_error().decode())
+
+
 @pytest.mark.gpu
 def test_more_packed_rows_than_a_launch_takes():
     """2^28 rows by workgroups of 16 and 2^27 by workgroups of 8 are 2^32 threads."""
