@@ -103,7 +103,7 @@ _KINDS = {**DTYPES, torch.int32: 32, torch.int64: 64}
 
 def _same(t: torch.Tensor, shape: tuple, kind: int, device: torch.device) -> torch.Tensor:
     """A tensor that the backward pass reads by address: as it was saved, but for its layout."""
-    if t.shape != shape or _KINDS.get(t.dtype) != kind or not t.is_cuda or t.device != device:
+    if t.shape != shape or _KINDS.get(t.dtype) != kind or t.device != device:
         raise RuntimeError(f"distill_topk_loss: a saved tensor came back as {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.contiguous()
 
@@ -135,12 +135,13 @@ class _Loss(torch.autograd.Function):
         # has made their device and the forward pass's stream the current ones.)
         z, ids, tv, lse, stats = ctx.saved_tensors
         dtype, rows, vocab, ld, bits, top, t = ctx.sizes
-        if z.shape != (rows, vocab) or DTYPES.get(z.dtype) != dtype or not z.is_cuda:
+        dev = z.device
+        if z.shape != (rows, vocab) or DTYPES.get(z.dtype) != dtype or dev != g.device:
             raise RuntimeError(f"distill_topk_loss: the logits came back as {tuple(z.shape)} {z.dtype} on {z.device}")
-        ids = _same(ids, (rows, top), bits, z.device)
-        tv, stats = _same(tv, (rows, top), _lib.LIRA_DTYPE_F32, z.device), _same(stats, (rows, 4), _lib.LIRA_DTYPE_F32, z.device)
+        ids = _same(ids, (rows, top), bits, dev)
+        tv, stats = _same(tv, (rows, top), _lib.LIRA_DTYPE_F32, dev), _same(stats, (rows, 4), _lib.LIRA_DTYPE_F32, dev)
         if lse is not None:
-            lse = _same(lse, (rows,), _lib.LIRA_DTYPE_F32, z.device)
+            lse = _same(lse, (rows,), _lib.LIRA_DTYPE_F32, dev)
         if z.stride() != (ld, 1):
             z, ld = _rows(z)
         if ctx.factor is not None:
@@ -148,10 +149,10 @@ class _Loss(torch.autograd.Function):
         whole = g.dim() == 0 or (rows > 1 and g.stride(0) == 0)  # one factor for all rows
         if not whole:
             g = g.contiguous()
-        dz = torch.empty((rows, vocab), dtype=z.dtype, device=z.device)
+        dz = torch.empty((rows, vocab), dtype=z.dtype, device=dev)
         _lib.run("lira_distill_topk_backward", z.data_ptr(), dtype, rows, vocab, ld, ids.data_ptr(), bits, tv.data_ptr(), top, t,
                  None if lse is None else lse.data_ptr(), stats.data_ptr(), g.data_ptr(), 0 if whole else 1, dz.data_ptr(),
-                 vocab, raw_stream(z.device.index))
+                 vocab, raw_stream(dev.index))
         return dz, None, None, None, None, None
 
 
@@ -191,7 +192,8 @@ def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_
     with on(dev, stream):
         z, lead, ids, tv, lse = _entries(logits, top_ids, top_logits, temperature, teacher_lse)
         w = _row_values(row_weight, "row_weight", lead, dev)
-        keep_for(stream, logits, top_ids, top_logits, teacher_lse, row_weight)
+        if stream is not None:
+            keep_for(stream, logits, top_ids, top_logits, teacher_lse, row_weight)
         z = _rows(z)[0]  # (perhaps a copy: held until the launch, the head has its address alone)
         if grad_out is None:
             dz = torch.empty(logits.shape, dtype=z.dtype, device=dev)
@@ -202,7 +204,8 @@ def distill_topk_loss_and_grad(logits: torch.Tensor, top_ids: torch.Tensor, top_
             dz = grad_out
             same = dz.data_ptr() == z.data_ptr() and z.is_contiguous()  # (the logits' own places)
             refuse_shared(dz, "grad_out (but for the logits themselves)", None if same else z, ids, tv, lse, w)
-            keep_for(stream, dz)
+            if stream is not None:
+                keep_for(stream, dz)
             increment_version(dz)  # (autograd may have saved it: the logits' own operation, where it is the logits)
         loss = _forward(_head(z, ids, tv, lse, temperature), dev, None, w, dz)
     return loss if len(lead) == 1 else loss.view(lead), dz

@@ -49,12 +49,11 @@ def on(device: torch.device, stream=None):
 def keep_for(stream, *tensors) -> None:
     """A call on a stream of its own: the memory that it reads or writes belongs to other streams, which must not give
     it out again before the call is through."""
-    if stream is not None:
-        for t in tensors:
-            if isinstance(t, MX4Tensor):
-                keep_for(stream, t._buf, t._codes, t._scales)
-            elif t is not None:
-                t.record_stream(stream)
+    for t in tensors:
+        if isinstance(t, MX4Tensor):
+            keep_for(stream, t._buf, t._codes, t._scales)
+        elif t is not None:
+            t.record_stream(stream)
 
 
 def check_rows(x, name: str, device=None) -> torch.Tensor:
@@ -227,7 +226,8 @@ def mx4_quantize(x: torch.Tensor, stream=None) -> MX4Tensor:
     p = (k + 127) // 128
     dev = x.device
     with on(dev, stream):
-        keep_for(stream, x)
+        if stream is not None:
+            keep_for(stream, x)
         x, ld = _rows(x)
         t = MX4Tensor._of(torch.empty(p * n * 68, dtype=torch.uint8, device=dev), n, k)
         _lib.run("lira_mx4_quantize", x.data_ptr(), DTYPES[x.dtype], n, k, ld, *t.addresses(), n,
@@ -259,7 +259,8 @@ def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float32, out: torch.
     dev, n = t.device, t.n
     with on(dev, stream):
         out, ld = _out(out, (n, t.k), dtype, dev, t)
-        keep_for(stream, t, out)
+        if stream is not None:
+            keep_for(stream, t, out)
         _lib.run("lira_mx4_dequantize", *t.addresses(), t.plane_rows, n, t.k, out.data_ptr(), DTYPES[dtype], ld,
                  raw_stream(dev.index))
     return out
@@ -294,10 +295,12 @@ def mx4_matmul(a: MX4Tensor, b: MX4Tensor, bias: torch.Tensor | None = None, act
     m, n = a.n, b.n
     dev = a.device
     with on(dev, stream):
-        keep_for(stream, a, b, bias)
+        if stream is not None:
+            keep_for(stream, a, b, bias)
         bias = None if bias is None else bias.to(torch.float32).contiguous()
         out, ldo = _out(out, (m, n), out_dtype, dev, a, b, bias)
-        keep_for(stream, out)
+        if stream is not None:
+            keep_for(stream, out)
         _lib.run("lira_mx4_matmul", *a.addresses(), a.plane_rows, m, *b.addresses(), b.plane_rows, n, a.k, alpha, _lib.ptr(bias), act, out.data_ptr(),
                  DTYPES[out_dtype], ldo, raw_stream(dev.index))
     return out
@@ -326,11 +329,13 @@ def mx4_linear(x: torch.Tensor, w: MX4Tensor, bias: torch.Tensor | None = None, 
     m, n, k, dev = x.shape[0], w.n, w.k, x.device
     need = _linear_workspace(m, n, k)
     with on(dev, stream):
-        keep_for(stream, x, w, bias)
+        if stream is not None:
+            keep_for(stream, x, w, bias)
         x, ld = _rows(x)
         bias = None if bias is None else bias.to(torch.float32).contiguous()
         out, ldo = _out(out, (m, n), out_dtype, dev, x, w, bias)
-        keep_for(stream, out)
+        if stream is not None:
+            keep_for(stream, out)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.run("lira_mx4_linear", x.data_ptr(), DTYPES[x.dtype], m, k, ld, *w.addresses(), w.plane_rows, n, alpha, _lib.ptr(bias), act, out.data_ptr(), DTYPES[out_dtype], ldo, _lib.ptr(ws), need,
                  raw_stream(dev.index))
