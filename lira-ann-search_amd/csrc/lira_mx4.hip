@@ -90,7 +90,8 @@ __device__ __forceinline__ void finish(f32x4 (&acc)[N], f32x4 bias, const Epilog
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[j][i] = acc[j][i] < 0.0f ? 0.0f : acc[j][i];  // (NaN stays NaN)
     } else if (e.act == LIRA_ACT_SIGMOID) {
-        // (hardware exp2 and reciprocal: 2 ulp of the exponent's rounding and 1 of the quotient's, under 2^-20)
+        // (hardware exp2 and reciprocal, 1 ulp each, and the exponent's rounding, which grows with the argument x: off by
+        // (1.5 |x| + 4) 2^-24 of the value, which is under 2^-21 absolutely, and 2^-17 of the value at x = -80)
 #pragma unroll
         for (int j = 0; j < N; ++j)
 #pragma unroll
@@ -755,7 +756,9 @@ static int product(const Product &p, hipStream_t st) {
 // tiles a compute unit that this takes no longer than a launch of its own does (kernels alone, fp32, us, packed here
 // and by themselves: 1000 x 256 x 128 5.2 and 5.2, 4000 x 1024 x 128 6.8 and 8.0, 50000 x 256 x 128 14.8 and 19.2,
 // 1000 x 1024 x 256 6.5 and 6.1; 1000 x 1024 x 384 9.3 and 6.4; a call from Python takes 4 less).  Rows that are not
-// aligned take 7.6 and 11.4, not 5.2 and 6.8.
+// aligned, 4-byte loads, take the same way, since the workspace's size goes by shapes alone, but a launch of their own
+// is faster: 1000 x 256 x 128 8.4 packed here and 5.8 by themselves, 4000 x 1024 x 128 12.6 and 8.4, 50000 x 256 x
+// 128 31.1 and 26.2, 1000 x 1024 x 256 12.4 and 6.7.
 static bool tile_packed(int64_t m, int64_t n, int64_t k) {
     const int64_t planes = planes_of(k), load = (((n + 127) / 128) * ((m + 63) / 64) + 255) / 256;
     return m > 16 && n >= 64 && k % 8 == 0 && planes <= 2 && load * planes <= 10;
