@@ -397,7 +397,7 @@ def run_workload(args, data, rank, world, gpu, dev, dist, primary):
         mfma_what = "bf16 MFMA" if split else "fp32 MFMA"
     else:
         flops = work["chunks_computed"] * dpad * 2
-        mfma_peak, mfma_what = MFMA_F32_PEAK_TFLOPS, "fp32 VALU (v_pk_fma_f32)"
+        mfma_peak, mfma_what = MFMA_F32_PEAK_TFLOPS, "fp32 VALU (v_fma_f32)"
     if kname == "k_screen_r":
         # L2 -> VGPR bytes per launch: per computed tile (64 candidates) their hi parts + xadj
         # (the work counter "blocks" counts tiles for this kernel)

@@ -9,7 +9,7 @@
 // scan VALU-bound at 3 ops/dim.  Here every candidate is first *screened* with
 // a dot product on the matrix cores -- by default bf16 parts of the (L2:
 // pivot-centred) vectors on v_mfma_f32_16x16x32_bf16 (k_screen_m, SPLIT 1-3;
-// the fp32 forms: v_mfma_f32_16x16x4_f32, or v_pk_fma_f32 in k_screen) -- and
+// the fp32 forms: v_mfma_f32_16x16x4_f32, or v_fma_f32 in k_screen) -- and
 // only the few candidates that can still reach the top-k are re-computed in the
 // reference's arithmetic (k_smerge).  Nothing is approximated: the screen is a
 // rigorous filter, so the output is bit-identical.  The error model below is
@@ -34,7 +34,7 @@
 // LDS ring by LDS-DMA; each wave owns RW = QR/4 query rows and all 256
 // candidates of a block (4 per lane); the rows' query values come from a
 // per-item transposed copy (k_qstage) through scalar loads, so the inner step
-// is one ds_read_b128 + RW*2 v_pk_fma_f32 with SGPR-broadcast operands.
+// is one ds_read_b128 + RW*4 v_fma_f32 with SGPR-broadcast operands.
 //
 // Selection per row: a sorted list of K2 = 32*RL >= k+8 screened keys
 // (s~ << 32 | storage row) in LDS with a 32-key survivor buffer (ballot
@@ -329,14 +329,15 @@ bool debug_build() { return false; }
 #define LIRA_SGLDS sglds16
 #endif
 
-// acc += x * splat(q.lo) / splat(q.hi) on packed fp32.  Inline asm: hipcc
-// otherwise copies every odd-register splat source with a v_mov first (one
-// extra VALU op per 8 FMAs), while op_sel reads either half in place.
-__device__ __forceinline__ void pkfma_lo(f2 &acc, f2 x, f2 q) {
-    asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel_hi:[1,0,1]" : "+v"(acc) : "v"(x), "v"(q));
+// acc += x * splat(q.lo) / splat(q.hi).  Two scalar FMAs: no packed fp32 instruction is used in
+// this library (the Makefile has the flag), some of their forms having given wrong results.
+__device__ __forceinline__ void fma2_lo(f2 &acc, f2 x, f2 q) {
+    acc.x = fmaf(x.x, q.x, acc.x);
+    acc.y = fmaf(x.y, q.x, acc.y);
 }
-__device__ __forceinline__ void pkfma_hi(f2 &acc, f2 x, f2 q) {
-    asm("v_pk_fma_f32 %0, %1, %2, %0 op_sel:[0,1,0] op_sel_hi:[1,1,1]" : "+v"(acc) : "v"(x), "v"(q));
+__device__ __forceinline__ void fma2_hi(f2 &acc, f2 x, f2 q) {
+    acc.x = fmaf(x.x, q.y, acc.x);
+    acc.y = fmaf(x.y, q.y, acc.y);
 }
 
 // the value lane 4 g + reg holds (lanes 0..15: one per query row), for every
@@ -587,14 +588,14 @@ __global__ __launch_bounds__(kSThreads, OCC) void k_screen(ScreenArgs a) {
                     for (int r4 = 0; r4 < RW / 4; ++r4) {
                         const f4 q4 = *(const f4 *)(qp + j * QR + r4 * 4);
                         const f2 q01 = q4.xy, q23 = q4.zw;
-                        pkfma_lo(acc[r4 * 4 + 0][0], xa, q01);
-                        pkfma_lo(acc[r4 * 4 + 0][1], xb, q01);
-                        pkfma_hi(acc[r4 * 4 + 1][0], xa, q01);
-                        pkfma_hi(acc[r4 * 4 + 1][1], xb, q01);
-                        pkfma_lo(acc[r4 * 4 + 2][0], xa, q23);
-                        pkfma_lo(acc[r4 * 4 + 2][1], xb, q23);
-                        pkfma_hi(acc[r4 * 4 + 3][0], xa, q23);
-                        pkfma_hi(acc[r4 * 4 + 3][1], xb, q23);
+                        fma2_lo(acc[r4 * 4 + 0][0], xa, q01);
+                        fma2_lo(acc[r4 * 4 + 0][1], xb, q01);
+                        fma2_hi(acc[r4 * 4 + 1][0], xa, q01);
+                        fma2_hi(acc[r4 * 4 + 1][1], xb, q01);
+                        fma2_lo(acc[r4 * 4 + 2][0], xa, q23);
+                        fma2_lo(acc[r4 * 4 + 2][1], xb, q23);
+                        fma2_hi(acc[r4 * 4 + 3][0], xa, q23);
+                        fma2_hi(acc[r4 * 4 + 3][1], xb, q23);
                     }
                 }
                 slot ^= 1;
@@ -1566,8 +1567,7 @@ __device__ __forceinline__ float seed_bound(const float *Q, const int32_t *probe
         const float qv = j0 + lane < d ? qrow[j0 + lane] : 0.0f;
         const int nj = (int)min<int64_t>(64, d - j0);
         if (nj == 64) {
-            // two tiles per packed fp32 op (v_pk_add_f32 / v_pk_mul_f32 round
-            // each half like the scalar ops: the same per-lane sums)
+            // two tiles a step (each half rounds like the scalar ops: the same per-lane sums)
             f2 acc2[NT / 2 > 0 ? NT / 2 : 1];
 #pragma unroll
             for (int t = 0; t < NT / 2; ++t) acc2[t] = (f2){acc[2 * t], acc[2 * t + 1]};
@@ -2629,7 +2629,7 @@ std::string screen_describe(const lira_index *idx, int64_t nq, int64_t nprobe, i
                                  : pl.split == 2 ? "k_screen_m hi-x split-bf16 v_mfma_f32_16x16x32_bf16"
                                  : pl.split ? "k_screen_m split-bf16 v_mfma_f32_16x16x32_bf16"
                                         : "k_screen_m fp32 v_mfma_f32_16x16x4_f32")
-                            : "k_screen VALU v_pk_fma_f32";
+                            : "k_screen VALU v_fma_f32";
     s += " RL=" + std::to_string(pl.rl) + " QR=" + std::to_string(pl.qr) + " K2=" + std::to_string(pl.K2) +
          (pl.rs ? " W=" + std::to_string(pl.waves) : std::string()) +
          " grid=" + std::to_string(pl.grid) + " smem=" + std::to_string(pl.smem);

@@ -8,7 +8,7 @@ root=$(cd "$(dirname "$0")/.." && pwd)
 pkg=$root/lira-ann-search_amd
 out=$root/variants/obj_$name
 mkdir -p "$out"
-F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -I$root/include -I$pkg/csrc $VARIANT_FLAGS"
+F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -Xclang -target-feature -Xclang -packed-fp32-ops -I$root/include -I$pkg/csrc $VARIANT_FLAGS"
 objs=""
 for s in "$pkg"/csrc/*.hip; do
   b=$(basename "$s")

@@ -9,7 +9,7 @@ root=$(cd "$(dirname "$0")/.." && pwd)
 pkg=$root/lira-ann-search_amd
 make -s -C "$pkg"
 mkdir -p "$root/variants/obj_$name"
-F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -I$root/include -I$pkg/csrc $VARIANT_FLAGS"
+F="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -Xclang -target-feature -Xclang -packed-fp32-ops -I$root/include -I$pkg/csrc $VARIANT_FLAGS"
 cp "$src" "$pkg/csrc/_variant.hip"
 /opt/rocm/bin/hipcc $F -c "$pkg/csrc/_variant.hip" -o "$root/variants/obj_$name/variant.o"
 rm -f "$pkg/csrc/_variant.hip"
