@@ -7,7 +7,7 @@ One step = one pass of the hot path over one batch of synthetic queries on
 every rank: MFMA ranking GEMM + exact nprobe boundary re-check
 (lira_rank_nearest) -> batched scan + exact top-k (lira_scan_topk) -> for
 N > 1 an RCCL all-gather of the per-rank top-k (every rank holds a full index
-replica; SURVEY.md 8(e)).  Inputs are resident in HBM before the timed region.
+replica).  Inputs are resident in HBM before the timed region.
 Rank 0 prints ONE JSON line (the bench contract).
 
 Scaling: ``weak`` (default) gives every rank its own batch of --nq queries;
@@ -24,8 +24,8 @@ queries / max-over-ranks time (strong scaling).
 Multi-GPU: `python bench.py --gpus N` with N > 1 and no WORLD_SIZE in the
 environment starts N ranks itself (a child `python -m torch.distributed.run
 --nproc-per-node N ... bench.py` process; this parent never touches the GPU and
-exits with the child's status).  Under torch.distributed.run (the driver's
-form) it runs as one of the ranks.  Every N > 1 line carries both figures:
+exits with the child's status).  Under torch.distributed.run (one rank a
+process) it runs as one of the ranks.  Every N > 1 line carries both figures:
 `value` for --scaling (weak by default) and an `other_scaling` sub-record for
 the other mode on the same index, plus `ranks_seen` (the world size the
 process group reported and each rank's device).
@@ -45,10 +45,10 @@ sys.path.insert(0, os.path.join(ROOT, "lira-ann-search_amd"))
 import numpy as np  # noqa: E402
 import torch  # noqa: E402
 
-# peaks (MI355X_MICROARCH.md)
+# peaks
 HBM_PEAK_GBS = 8000.0          # HBM3E spec
 L2LDS_PEAK_GBS = 18800.0       # LDS-DMA gather into LDS from the XCD L2, chip-wide (upper end, measured)
-L2_PEAK_GBS = 34500.0          # L2 read bandwidth, chip-wide (MI355X_MICROARCH.md, L2 per XCD)
+L2_PEAK_GBS = 34500.0          # L2 read bandwidth, chip-wide (of the 8 XCDs together)
 MFMA_F32_PEAK_TFLOPS = 157.3   # v_mfma_f32_*_f32 dense = fp32 vector peak
 MFMA_BF16_PEAK_TFLOPS = 2516.6  # dense bf16 MFMA, 16 x the f32 rate
 VALU_F32_PEAK_TOPS = 78.64     # non-FMA fp32 lane ops/s (157.3 TFLOP/s counts an FMA as 2)
@@ -68,7 +68,7 @@ def parse():
     ap.add_argument("--fma", action="store_true",
                     help="LIRA_SCAN_FMA accumulation (tolerance variant, not the reference's rounding)")
     ap.add_argument("--data", default="mixture", choices=["latent", "mixture", "uniform"],
-                    help="synthetic distribution (lira_amd/synthetic.py): mixture = SURVEY 8(d)'s "
+                    help="synthetic distribution (lira_amd/synthetic.py): mixture = the "
                          "Gaussian mixture (default); latent = low intrinsic dimension + k-means "
                          "partitions, recall near the metric's 0.95 point like real SIFT1M")
     ap.add_argument("--contrast", default="auto", choices=["auto", "none"],
@@ -434,7 +434,7 @@ def run_workload(args, data, rank, world, gpu, dev, dist, primary):
         c["frac"] = c["achieved"] / c["peak"]
     binding = max(cands, key=lambda n: cands[n]["frac"])
     bc = cands[binding]
-    eff_bytes = cand * d * 4 + nq * (4 * d + 12 * k)  # SURVEY 8(d) per-launch algorithmic bytes
+    eff_bytes = cand * d * 4 + nq * (4 * d + 12 * k)  # algorithmic bytes a launch: every probed candidate once a query
     out["roofline"] = {
         "bound": "mfma" if binding == "mfma" else "hbm", "binding": binding,
         "achieved": bc["achieved"], "peak": bc["peak"], "unit": bc["unit"], "frac": bc["frac"],
@@ -601,7 +601,7 @@ def run_workload(args, data, rank, world, gpu, dev, dist, primary):
             cb["blas_form"] = {"value": blas_qps, "sample": cb["sample"], "seconds": bs,
                                "topk_agreement_with_gpu": agree}
             cb.update(value=scalar["value"], sample=scalar["sample"], seconds=scalar["seconds"])
-    # ---- the MLP-probed search.cpp pipeline, N = 1 ---------------
+    # ---- the MLP-probed search.cpp pipeline, N = 1 ---------------------------------
     if primary and world == 1 and B <= 256 and not args.no_pipeline:
         out["pipeline"] = time_pipeline(args, oracle, index, x, centres, q, make_queries, k, nprobe, metric,
                                         host, rows, Igt, dev)
@@ -989,7 +989,7 @@ def main():
         torch.cuda.empty_cache()
         other = "latent" if args.data != "latent" else "mixture"
         contrast = run_workload(args, other, rank, world, gpu, dev, dist, primary=False)
-        if args.config == "sift1m" and args.data != "uniform":  # north_star's literal random-float vectors
+        if args.config == "sift1m" and args.data != "uniform":  # i.i.d. random-float vectors
             torch.cuda.empty_cache()
             contrast_u = run_workload(args, "uniform", rank, world, gpu, dev, dist, primary=False)
 

@@ -14,8 +14,8 @@
  * are stream-ordered and asynchronous unless stated otherwise.
  *
  * What each entry point replaces in the reference (qfshen23/LIRA-ANN-search,
- * file:line) is stated above it.  INTEGRATION.md shows the ctypes binding the
- * reference's Python side would use, and lira_amd/_lib.py is that binding.
+ * file:line) is stated above it.  lira_amd/_lib.py is the ctypes binding that the
+ * reference's Python side would use.
  */
 #ifndef LIRA_HIP_H
 #define LIRA_HIP_H
@@ -45,8 +45,8 @@ extern "C" {
 /* lira_scan_topk flags */
 #define LIRA_SCAN_DEDUP 1u         /* keep each gid once (search.cpp:496-514 does not: Appendix A) */
 #define LIRA_SCAN_PER_PARTITION 2u /* k best of every probed slot on its own (LIRA_smallscale.py:145-174) */
-#define LIRA_SCAN_FMA 4u           /* fused multiply-add accumulation: fewer ops, NOT bit-exact (SURVEY 7
-                                      "tolerance fallback": 1e-4 relative, ties may order differently) */
+#define LIRA_SCAN_FMA 4u           /* fused multiply-add accumulation: fewer ops, NOT bit-exact (a
+                                      tolerance of 1e-4 relative, ties may order differently) */
 #define LIRA_SCAN_NO_PRUNE 8u      /* L2: compute every candidate to the last dim (no early abandon of
                                       pairs already past the k-th score); same results, for A/B */
 #define LIRA_SCAN_EXACT 16u        /* use the all-exact scan (every candidate in search.cpp's arithmetic)
@@ -201,7 +201,7 @@ int lira_index_memory(const lira_index *idx, int64_t *bytes);
  *                        wave-streaming screen k_screen_r takes IP as q.x = q.fl(x - c) + q.c with a
  *                        Cauchy-Schwarz block skip (k <= 120, dpad <= 128); needs
  *                        LIRA_OPT_KEEP_TILES = 1 (the other screens read the fp32 tiles on such an
- *                        index).  0: the uncentred split copy (round-4 layout).  Results never
+ *                        index).  0: the uncentred split copy (the older layout).  Results never
  *                        depend on it.
  *   LIRA_OPT_CHUNK       screen work items: at most this many blocks of 256 candidates per chunk
  *                        of a bucket (0, default: the plan's choice, <= 128).  Results never
@@ -240,7 +240,7 @@ int lira_index_has_tiles(const lira_index *idx, int *out);
 /* ------------------------------------------------- partition shards */
 /*
  * k-way merge of per-shard top-k results: the exchange step of the
- * partition-sharded search (SURVEY.md 8(e): each rank holds the lists of its
+ * partition-sharded search (each rank holds the lists of its
  * own buckets, scans them for every query, and the ranks' (nq, k) results are
  * all-gathered and merged).  Each shard's lists hold a disjoint set of
  * (bucket, row) entries, so the k smallest keys of the union equal the
@@ -452,7 +452,7 @@ int lira_distill_reduce(const float *loss, const float *stats, int64_t rows, int
  * capture); a cached buffer that a captured graph uses is kept allocated when a
  * later eager call outgrows it (until lira_index_destroy), so replays stay valid.
  *
- * Threading and streams (SURVEY 8(b)).  Calls are asynchronous and stream-
+ * Threading and streams.  Calls are asynchronous and stream-
  * ordered.  Several streams (and host threads) may search ONE handle at the same
  * time: the cached workspace is kept per stream (the plan counters, item tables,
  * row lists and bounds of one call are never shared with another stream's call),

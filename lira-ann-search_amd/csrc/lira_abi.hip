@@ -824,7 +824,7 @@ int lira_index_set_option(lira_index *idx, int option, int64_t value) {
         case LIRA_OPT_TWO_PHASE: if (!in(0, 2)) break; o.two_phase = v; return LIRA_OK;
         case LIRA_OPT_PRUNE: if (!in(0, 1)) break; o.prune = v; return LIRA_OK;
         case LIRA_OPT_SEED:
-            if (value == 2 || value == 3)  // (k_seed_b, measured slower: removed in round 4)
+            if (value == 2 || value == 3)  // (k_seed_b, measured slower: removed)
                 return fail(LIRA_EUNSUPPORTED, "LIRA_OPT_SEED 2 / 3 (block-shared seed) was removed");
             if (!in(0, 1)) break;
             o.seed = v;
@@ -838,7 +838,7 @@ int lira_index_set_option(lira_index *idx, int option, int64_t value) {
             if (v && !debug_build())  // a production build never returns invalid results
                 return fail(LIRA_EUNSUPPORTED, "LIRA_OPT_DEBUG needs a library built with -DLIRA_DEBUG");
             o.debug = v; return LIRA_OK;
-        case LIRA_OPT_PIPELINE:  // (k_screen_s, k_screen_w, k_screen_v: measured slower, removed in round 4)
+        case LIRA_OPT_PIPELINE:  // (k_screen_s, k_screen_w, k_screen_v: measured slower, removed)
         case LIRA_OPT_RING:
         case LIRA_OPT_WIDE:
             if (value == 0) return LIRA_OK;

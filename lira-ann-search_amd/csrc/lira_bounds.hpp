@@ -1,6 +1,6 @@
 // lira_bounds.hpp -- the screen's rigorous error model (double precision),
 // shared by the screening kernels (lira_screen.hip, lira_wscreen.hip).  The
-// derivation is in lira_screen.hip's header and DESIGN.md section 4.3.
+// derivation is in lira_screen.hip's header.
 #pragma once
 #include "lira_device.hpp"
 

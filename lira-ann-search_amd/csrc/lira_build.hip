@@ -1,4 +1,4 @@
-// lira_build.hip -- device-side inverted-list builder (SURVEY.md 8(f) row 1).
+// lira_build.hip -- device-side inverted-list builder.
 //
 // Replaces search.cpp:366-385: for every row i and slot j of data_2_bkt
 // (N, n_mul; -1 = empty), bucket data_2_bkt[i][j] receives row i; each bucket's

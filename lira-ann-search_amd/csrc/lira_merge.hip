@@ -1,5 +1,5 @@
 // k-way merge of per-shard top-k lists: the exchange step of the partition-
-// sharded search (SURVEY.md 8(e), "shard by partition ... all-gather 8 x (nq, k)
+// sharded search ("shard by partition ... all-gather 8 x (nq, k)
 // and k-way merge").  Each rank scans only the lists it owns for every query;
 // its (nq, k) result is the exact top-k over its candidates, so the k smallest
 // (score, id) keys of the union of the P ranks' lists are the single-GPU

@@ -423,7 +423,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 1 : 2) void k_screen_r(RArgs a) {
         // B operands: a ring of NC chunks of [candidate group] -- the whole next
         // tile: chunk c's slot is reloaded with the next tile's chunk c as soon as its
         // MFMAs have issued, so a tile's loads have a whole tile (MFMAs + selection)
-        // to land (two chunks ahead, round 4's ring at d = 128, left chunks 2-3 of
+        // to land (two chunks ahead, the first ring at d = 128, left chunks 2-3 of
         // every tile waiting on HBM).  The wave's first tile is requested before the
         // prologue (under its loads and barriers), and again only if skipped.
         // (NC = 0: dpad > 128, the dims streamed two chunks ahead -- a whole tile is

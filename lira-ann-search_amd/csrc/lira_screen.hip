@@ -2454,11 +2454,11 @@ static SPlan make_splan(const lira_index *idx, int64_t nq, int64_t nprobe, int64
     // against the score spread)
     if (pl.split && xhi && pl.qr != 32 && pl.rl <= (pl.qr == 64 ? 4 : 1)) pl.split = 2;
     if (pl.split == 2 && xhi == 2 && pl.qr == 64 && pl.rl == 1) pl.split = 3;
-    // (round 3 measured a pipelined NS-slot ring screen, k_screen_s, slower on
-    // every config -- DEEP10M 28.1 vs 24.9 ms; removed in round 4, git history keeps it)
+    // (a pipelined NS-slot ring screen, k_screen_s, was slower on
+    // every config -- DEEP10M 28.1 vs 24.9 ms; removed, git history keeps it)
     pl.K2 = 32 * pl.rl;
     // (the wide k_screen_w and wave-resident k_screen_v screens measured 0.571 /
-    // 1.50 ms against 0.325 on SIFT1M: removed in round 4)
+    // 1.50 ms against 0.325 on SIFT1M: removed)
     pl.pp = pl.split == 3;
     // k_screen_r where it applies (its own preconditions on the scan's flags are in screen_topk)
     // (with or without the fp32 tiles: the seed then comes from the row-major copy
@@ -2511,7 +2511,7 @@ static SPlan make_splan(const lira_index *idx, int64_t nq, int64_t nprobe, int64
     // per workgroup left the slowest workgroup with two (LIRA_OPT_NEAR_ROUNDS;
     // measured SIFT1M mixture scan 1.08 -> 1.04 ms at 2, slower at 4 and 8:
     // more lists, more survivors)
-    // (1 since round 4 for k_screen_m too, with its group-0 chunks fixed: DEEP10M scan
+    // (1 for k_screen_m too, with its group-0 chunks fixed: DEEP10M scan
     // 22.2 -> 21.5 ms, merge 0.32 -> 0.26 ms; GIST1M mixture scan -2 %, latent even)
     const int near_rounds = op.near_rounds > 0 ? op.near_rounds : 1;
     {
@@ -2551,7 +2551,7 @@ static SPlan make_splan(const lira_index *idx, int64_t nq, int64_t nprobe, int64
         pl.bpc_near_min = (int)std::min<int64_t>(pl.bpc_near, std::max<int64_t>(1, (max_blocks + split6 - 1) / split6));
     }
     // (k_screen_r) group 0's small first chunks, waited for by the query block's others
-    // (default 4 blocks since round 6: SIFT1M mixture scan 0.221 -> 0.219 ms, latent equal,
+    // (default 4 blocks: SIFT1M mixture scan 0.221 -> 0.219 ms, latent equal,
     // DEEP10M mixture 1.634 -> 1.600; 6 was slower on SIFT1M)
     if (pl.rs && two) {
         const int nf = op.near_first < 0 ? 4 : op.near_first;

@@ -1,7 +1,7 @@
 """ctypes binding of liblira_hip.so (include/lira_hip.h).
 
 This is the binding the reference's Python side would add to reach the HIP
-module (INTEGRATION.md).  There is no fallback: if the shared library is
+module.  There is no fallback: if the shared library is
 missing or cannot be loaded, every entry point raises ``LiraError`` -- the hot
 path never silently runs on the CPU or in plain PyTorch.
 """

@@ -1,4 +1,4 @@
-"""Query-sharded multi-GPU search (SURVEY.md 8(e)).
+"""Query-sharded multi-GPU search.
 
 Queries are independent, so a batch is split into contiguous slices, one per
 rank (one process per GPU, torch.distributed over RCCL -- backend "nccl" on
@@ -8,7 +8,7 @@ all-gathered so every rank (the caller on rank 0 in particular) sees the whole
 batch's results.  That all-gather is the path's only exchange step: 12 bytes x
 k per query (1.2 MB for 10k queries at k=10), far below xGMI link rates.
 
-Partition sharding (SURVEY.md 8(e)'s alternative for BIGANN's memory): rank r
+Partition sharding (the alternative for BIGANN's memory): rank r
 holds only the lists of the buckets `partition_owners` gives it (balanced by
 list size), every rank ranks and scans the WHOLE query batch against its own
 lists (a probe into another rank's bucket finds an empty list), and the ranks'
@@ -16,7 +16,7 @@ lists (a probe into another rank's bucket finds an empty list), and the ranks'
 (lira_merge_shards).  The lists of different ranks are disjoint, so the merge
 of the per-rank exact top-k is the single-index result bit for bit.
 
-The reference has no distributed code (single GPU chosen by
+The reference has no distributed code (a single GPU chosen by
 nvidia-smi, utils.py:90-96); this module is new.
 """
 from __future__ import annotations

@@ -1,5 +1,4 @@
-"""Offline exhaustive self-kNN and k-means assignment on the HIP scan
-(SURVEY.md 8(f) row 4).
+"""Offline exhaustive self-kNN and k-means assignment on the HIP scan.
 
 Replaces, with the same inputs, outputs and on-disk contract:
 

@@ -104,7 +104,7 @@ class NearestCentroidProbe(nn.Module):
 
     With scaler mean 0 / scale 1 and a threshold in (0, 1], the threshold probe
     of search.cpp:447-466 then selects exactly the IVF nprobe nearest centroids
-    (the oracle construction of SURVEY.md 8(c)).  Ties at the boundary score 1.
+    (the oracle's construction).  Ties at the boundary score 1.
     """
 
     def __init__(self, nprobe: int):

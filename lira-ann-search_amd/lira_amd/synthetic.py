@@ -1,4 +1,4 @@
-"""Synthetic inputs of the BASELINE.json shapes.
+"""Synthetic inputs of the benchmark's shapes.
 
 Two distributions, both fp32:
 
@@ -11,15 +11,15 @@ Two distributions, both fp32:
   nprobe (nearest centroids) lands near the metric's 0.95 operating point
   (measured: SIFT1M m=12 -> 0.97, GIST1M m=16 -> 0.96, DEEP10M m=20 -> 0.985),
   as it does on the real datasets.  deep10m rows are L2-normalised (DEEP1B is).
-* ``uniform``: x ~ U[0, 1)^d i.i.d. (north_star's literal "synthetic random-float
+* ``uniform``: x ~ U[0, 1)^d i.i.d. ("synthetic random-float
   vectors"), k-means partitions like ``latent``.  No cluster structure: recall@k at
-  nprobe << B is low against global ground truth (hard part 7), so
+  nprobe << B is low against global ground truth, so
   it is a throughput and parity workload -- both sides scan identical probe lists.
 * ``mixture``: B centres ~ N(0,1)^d, point = centre[uniform label] +
   sigma * N(0,1)^d (sigma = 0.35), nearest-centre partitions.  In high d these
   clusters are perfectly separated (recall 1.0 at any nprobe >= 1), so exact
   pruning skips nearly every non-nearest partition: an easy best case.  It is
-  SURVEY.md 8(d)'s prescribed distribution, so bench.py's headline uses it
+  the prescribed distribution, so bench.py's headline uses it
   and reports the ``latent`` run beside it (``contrast_data``).
 """
 from __future__ import annotations
@@ -28,7 +28,7 @@ import numpy as np
 import torch
 
 CONFIGS = {
-    # name: (N, d, B, nprobe, k, metric, nq)  (BASELINE.json configs)
+    # name: (N, d, B, nprobe, k, metric, nq)
     "sift1m": (1_000_000, 128, 64, 8, 10, "L2", 10_000),
     "gist1m": (1_000_000, 960, 128, 16, 10, "L2", 1_000),
     "deep10m": (10_000_000, 96, 256, 32, 100, "inner_product", 10_000),

@@ -1,6 +1,6 @@
 """LIRA's query-path helpers (utils.py, LIRA_smallscale.py) on the HIP module.
 
-Same names and argument meaning as the reference, so a driver written against
+Same names and argument meaning as the reference, so a program written against
 LIRA's utils switches by import:
 
     get_dist_cid            utils.py:98-118          query->centroid distances
@@ -11,7 +11,7 @@ LIRA's utils switches by import:
     get_knn_distr_redundancy utils.py:354-379        gt neighbours per bucket (host)
     query_tuning            LIRA_smallscale.py:176-241   threshold sweep (host)
 
-Differences, all deliberate and documented in DESIGN.md:
+Differences, all deliberate:
 * distances are fp32 in search.cpp's sequential order (scipy's cdist works in
   float64 and casts; the two agree to ~1 ulp of the float32 result);
 * get_cmp_recall runs ONE batched scan of every bucket for every query instead

@@ -16,19 +16,19 @@
  *   oracle_build_csr          search.cpp:366-385  bucket -> sorted unique gids
  *   oracle_probe_threshold    search.cpp:447-466  score >= thr, argmax fallback
  *                             LIRA_smallscale.py:206 (score > thr, no fallback)
- *   oracle_probe_nearest      IVF nprobe (SURVEY.md 8(c) "nearest-nprobe" probe)
+ *   oracle_probe_nearest      IVF nprobe ("nearest-nprobe" probe)
  *   oracle_scan_topk          search.cpp:471-514  scan + top-k, canonical order
  *   oracle_scan_per_partition LIRA_smallscale.py:145-174 (per (q, bucket) top-k)
  *
  * Numerics: must be compiled with -ffp-contract=off (see oracle/Makefile) so
  * that `acc += diff * diff` rounds the product before the add, exactly like
- * the reference binary (SURVEY.md 3.1: subps/mulps then sequential addss).
+ * the reference binary (subps/mulps then sequential addss).
  *
  * Canonical top-k order: ascending (score, gid) where score = l2_sq for L2
  * and score = -ip for inner product (search.cpp:483-488).  The reference's
  * nth_element output is unordered and breaks boundary ties arbitrarily; this
  * restatement fixes the order so set equality with the reference holds
- * whenever the k-th boundary is not a tie (SURVEY.md Appendix A).
+ * whenever the k-th boundary is not a tie.
  */
 #include <math.h>
 #include <stdint.h>
