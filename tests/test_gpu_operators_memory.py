@@ -235,7 +235,7 @@ def test_memory_read_on_another_stream_is_not_given_out_again(name):
     side.wait_stream(torch.cuda.current_stream())
     torch.cuda.synchronize()
     with torch.cuda.stream(side):
-        torch.cuda._sleep(50_000_000)  # (half a second at most; the call waits behind it)
+        torch.cuda._sleep(500_000_000)  # (0.2 s; the call waits behind it)
     kept = []
     result = call(side, *inputs)
     held = [b for t in inputs for b in ((t._buf,) if isinstance(t, MX4Tensor) and t._buf is not None else
